@@ -36,6 +36,7 @@ extern "C" {
 /* Device-side status word values (written to `status` when non-NULL). */
 #define QIK_STATUS_OK 0
 #define QIK_STATUS_TIMEOUT 1
+#define QIK_STATUS_BAD_INDEX 2 /* a position, slot, page or length outside its tensor (skipped) */
 
 /* Library version (major*10000 + minor*100 + patch). */
 int qik_version(void);
@@ -470,6 +471,126 @@ int qik_tp_wait(const uint32_t* gcnt, uint32_t target, int world, int* status, v
  */
 int qik_rows_bias_bf16(const float* x, int64_t rows, int64_t N, const void* bias, void* out, uint32_t* amax_out,
                        void* stream);
+
+/*
+ * Residual addition + RMS norm of a transformer decoder, next to qik_rms_norm_rope and
+ * qik_layer_norm_modulate (the reference has no such operator):
+ *   h = x + residual (fp32; residual NULL: h = x);  sum_out = h rounded (NULL: not stored);
+ *   y = h * rsqrt(mean(h^2) + eps) * weight, from the unrounded h, rounded once into out.
+ *   x, residual [M, N] 16-bit with row pitches ldx, ldr (elements); bf16, or fp16 when
+ *   f16 != 0; weight [N] of the same type, or fp32 when weight_f32 != 0; out, sum_out
+ *   [M, N] contiguous.  N a multiple of 8, at most 32768; pitches multiples of 8; every
+ *   pointer 16-byte aligned.  A NULL residual with a NULL sum_out is the plain norm.
+ */
+int qik_add_rms_norm(const void* x, int64_t ldx, const void* residual, int64_t ldr, const void* weight,
+                     int weight_f32, int64_t M, int64_t N, float eps, int f16, void* sum_out, void* out,
+                     void* stream);
+
+/*
+ * The same with y quantized: scale = max(max|y| * fl32(1/448), 1e-12) over each row
+ * (row_scales != 0: scale [M]) or over the whole tensor (scale [1], the dynamic scale
+ * that qik_fp8_gemm takes), q [M, N] = e4m3 (nearest even) of y / scale.  y is not
+ * rounded to 16 bits in between; NaN in a row reaches its scale.
+ *   ws: qik_add_rms_norm_workspace_bytes(M) bytes, 16-byte aligned, not initialised by
+ *   the caller (whole-tensor scale only; NULL for row scales).  The whole-tensor form
+ *   reads x and residual twice: sum_out must not overlap them.
+ */
+size_t qik_add_rms_norm_workspace_bytes(int64_t M);
+int qik_add_rms_norm_e4m3(const void* x, int64_t ldx, const void* residual, int64_t ldr, const void* weight,
+                          int weight_f32, int64_t M, int64_t N, float eps, int f16, void* sum_out, void* q,
+                          float* scale, int row_scales, void* ws, void* stream);
+
+/*
+ * Rotary positions of q and k, optionally storing the rotated k and v into cache pages.
+ * The first `rot` columns of every q and k head are turned by the angles of row
+ * positions[t] of the tables cos / sin [P, rot / 2] (fp32): pairs (2i, 2i + 1) with
+ * QIK_ROTARY_INTERLEAVED, (i, i + rot / 2) without; the other columns are copied.
+ *   q [T, HQ, D], k [T, HK, D], v [T, HK, D] with element strides (token, head) and a
+ *   unit column stride; q_out [T, HQ, D] contiguous.
+ *   Without QIK_ROTARY_PAGED: k_out [T, HK, D] contiguous, v unused.
+ *   With it: token t's k and v go to page slots[t] / page, place slots[t] % page of k_out
+ *   / v_out (element strides page, head, token); a negative slot stores nothing (padding);
+ *   slots of one call are distinct.
+ *   positions, slots: int32, or int64 with QIK_ROTARY_POS64 / QIK_ROTARY_SLOT64.
+ * A position outside [0, P) gives zeros in q_out (and in k_out, or stores nothing), a slot
+ * behind the last page stores nothing; both set QIK_STATUS_BAD_INDEX in *status.
+ * D 64, 128 or 256; rot a multiple of 16, at most D; strides multiples of 8 elements;
+ * pointers 16-byte aligned.
+ */
+#define QIK_ROTARY_INTERLEAVED 1
+#define QIK_ROTARY_F16 2
+#define QIK_ROTARY_PAGED 4
+#define QIK_ROTARY_POS64 8
+#define QIK_ROTARY_SLOT64 16
+typedef struct {
+  const void *q, *k, *v;
+  void *q_out, *k_out, *v_out;
+  const void *positions, *slots;
+  const float *cos, *sin;
+  int64_t T, HQ, HK, D, rot, P;
+  int64_t q_st, q_sh, k_st, k_sh, v_st, v_sh;
+  int64_t page, pages;
+  int64_t kp_s0, kp_sh, kp_ss, vp_s0, vp_sh, vp_ss;
+  int flags;
+} qik_rotary_args;
+int qik_rotary(const qik_rotary_args* args, int* status, void* stream);
+
+/*
+ * Copies between pages of a paged KV cache: for each move (from, to, tokens) of the host
+ * array `moves` (3 int32 each) the first `tokens` tokens of page `from` are copied to page
+ * `to`, for every layer and head, in the k and in the v pool; the rest of page `to` stays.
+ * The list is checked before anything is launched: every index in range, no page
+ * written twice, none both read and written.  It is read during the call only.
+ *   pools: k, v: [layers][pages][heads][page][token_bytes] with byte strides for layer,
+ *   page and head; the tokens of a head are contiguous.  Strides, token_bytes and
+ *   pointers are multiples of 16 bytes.
+ */
+typedef struct {
+  void *k, *v;
+  int64_t layers, pages, heads, page, token_bytes;
+  int64_t k_layer_bytes, k_page_bytes, k_head_bytes;
+  int64_t v_layer_bytes, v_page_bytes, v_head_bytes;
+} qik_page_pools;
+int qik_copy_pages(const qik_page_pools* pools, const int32_t* moves, int64_t n, void* stream);
+
+/*
+ * Attention of new tokens over a paged KV cache, next to qik_block_causal_attention
+ * (one slab, equal query and key heads).  Sequence i has seq_lens[i] tokens in the cache,
+ * of which the last n_i = query_starts[i + 1] - query_starts[i] are new: rows
+ * query_starts[i] .. of q and out, in order, their k and v already stored.  Its token t is in
+ * page page_table[i, t / page], place t % page.
+ *   A new token at place p of its sequence sees the keys t <= p (QIK_PAGED_CAUSAL) or all
+ *   seq_lens[i] of them; with window > 0 (causal only) those with t > p - window or
+ *   t < sinks.  out = softmax(q . k * sm_scale) . v; a row that sees no key is 0.  Whatever
+ *   the unseen places of a page hold has no effect where no row of the call's sequence
+ *   sees them.
+ *   q, out [T, HQ, D] with element strides (token, head); k_pages, v_pages [pages, HK, page,
+ *   D] with element strides (page, head, token); unit column strides; bf16, or fp16 with
+ *   QIK_PAGED_F16; query head h reads key head h / (HQ / HK).  page_table [B, W] int32
+ *   with row stride table_st.  Rows of out behind query_starts[B] are not written.
+ *   max_new, max_kv: upper bounds (host) of n_i and seq_lens[i]; they choose launch shapes,
+ *   and no sequence may exceed max_new.
+ *   ws: qik_paged_attention_workspace_bytes(args) bytes, 16-byte aligned, not initialised by
+ *   the caller and free again when the call's kernels are done (0 bytes: NULL).
+ *   Lengths, starts and pages outside their tensors read zeros in their place and set
+ *   QIK_STATUS_BAD_INDEX in *status.
+ * D 64 or 128; page a power of two from 16 to 4096; strides multiples of 8 elements;
+ * pointers 16-byte aligned; sm_scale positive.
+ */
+#define QIK_PAGED_CAUSAL 1
+#define QIK_PAGED_F16 2
+typedef struct {
+  const void *q, *k_pages, *v_pages;
+  void* out;
+  const int32_t *page_table, *seq_lens, *query_starts;
+  int64_t B, T, HQ, HK, D, W, pages, page, max_new, max_kv;
+  int64_t q_st, q_sh, o_st, o_sh, table_st;
+  int64_t kp_s0, kp_sh, kp_ss, vp_s0, vp_sh, vp_ss;
+  float sm_scale;
+  int window, sinks, flags;
+} qik_paged_attn_args;
+size_t qik_paged_attention_workspace_bytes(const qik_paged_attn_args* args);
+int qik_paged_attention(const qik_paged_attn_args* args, void* ws, size_t ws_bytes, int* status, void* stream);
 
 /*
  * Self-test of the bounded-wait machinery: launches one CTA that waits on an

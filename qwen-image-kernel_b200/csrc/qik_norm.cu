@@ -1,0 +1,315 @@
+// qik_norm.cu -- residual addition + RMS norm, with a 16-bit output or e4m3 codes and
+// their scales.
+//
+//   h = x + r            (fp32; stored once, rounded to the tensors' type, as the new
+//                         residual stream; r may be absent: h = x)
+//   y = h * rsqrt(mean_cols(h^2) + eps) * w      (from the unrounded fp32 h)
+//   plain:   y rounded once to the tensors' type
+//   e4m3:    s = max(max|y| / 448, 1e-12) over the row or over the whole tensor,
+//            codes = e4m3(y / s), nearest even; no 16-bit y exists in between
+//
+// Bound by HBM: 6 bytes an element in and out for h (x, r, h) and 1 or 2 for y.  A row
+// is held in registers by one CTA between its load and its store, so a row's statistics
+// cost no second read.  The whole-tensor scale needs every row's maximum before the
+// first code: one kernel stores h, each row's 1 / rms and each CTA's max|y|, a second
+// (its programmatic dependent) forms the same y from x and r again and packs it.
+#include "qik_device.cuh"
+#include "qik_host.h"
+
+namespace qik {
+
+constexpr int kNormMaxSlots = 2048;  // CTAs of the first kernel, each with one max|y|
+
+struct NormDev {
+  const void* x;
+  const void* r;
+  const void* w;
+  void* h;
+  void* y;           // 16-bit output (plain) or e4m3 codes
+  float* scale;      // [M] (row scales) or [1]
+  float* rstd;       // [M] workspace (whole-tensor scale)
+  uint32_t* slots;   // [slot count] workspace: max|y| bits of each CTA of the first kernel
+  int64_t M, ldx, ldr;
+  int N, n_slots;
+  float eps;
+};
+
+enum NormMode { kNormPlain = 0, kNormRow = 1, kNormStats = 2 };
+
+template <bool F16>
+__device__ __forceinline__ void unpack8(const uint4 v, float (&f)[8]) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (F16) {
+      const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+      f[2 * i] = p.x;
+      f[2 * i + 1] = p.y;
+    } else {
+      f[2 * i] = __uint_as_float(w[i] << 16);
+      f[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+    }
+  }
+}
+template <bool F16>
+__device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] = F16 ? pack_f16x2(f[2 * i], f[2 * i + 1]) : pack_bf16x2(f[2 * i], f[2 * i + 1]);
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+template <bool F16, bool WF32>
+__device__ __forceinline__ void load_weight8(const void* w, int vec, float (&f)[8]) {
+  if (WF32) {
+    const float4* p = reinterpret_cast<const float4*>(w) + 2 * static_cast<int64_t>(vec);
+    const float4 a = __ldg(p), b = __ldg(p + 1);
+    f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
+  } else {
+    unpack8<F16>(__ldg(reinterpret_cast<const uint4*>(w) + vec), f);
+  }
+}
+__device__ __forceinline__ uint2 codes8(const float (&y)[8], float inv) {
+  uint32_t o[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    o[i] = static_cast<uint32_t>(cvt_e4m3x2(y[4 * i] * inv, y[4 * i + 1] * inv)) |
+           (static_cast<uint32_t>(cvt_e4m3x2(y[4 * i + 2] * inv, y[4 * i + 3] * inv)) << 16);
+  return make_uint2(o[0], o[1]);
+}
+// |y| as bits: non-negative floats order like their bits, and NaN lies above infinity,
+// so a maximum over bits lets a NaN through to the scale.
+__device__ __forceinline__ uint32_t abs_bits(float y) { return __float_as_uint(y) & 0x7FFFFFFFu; }
+
+// Block-wide sum (IsMax: maximum of bits) with one barrier: `buf` alternates between two
+// halves from call to call, so a fast warp's next write cannot overtake a slow warp's read.
+template <bool IsMax>
+__device__ __forceinline__ uint32_t block_reduce(uint32_t v, uint32_t* buf) {
+  const int warps = blockDim.x >> 5;
+  if (IsMax) {
+    v = __reduce_max_sync(0xffffffffu, v);
+  } else {
+    float f = __uint_as_float(v);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) f += __shfl_xor_sync(0xffffffffu, f, o);
+    v = __float_as_uint(f);
+  }
+  if ((threadIdx.x & 31) == 0) buf[threadIdx.x >> 5] = v;
+  __syncthreads();
+  uint32_t t = static_cast<int>(threadIdx.x & 31) < warps ? buf[threadIdx.x & 31] : 0u;
+  if (IsMax) return __reduce_max_sync(0xffffffffu, t);
+  float f = __uint_as_float(t);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) f += __shfl_xor_sync(0xffffffffu, f, o);
+  return __float_as_uint(f);
+}
+
+// One CTA walks rows blockIdx.x, + gridDim.x, ...; thread t holds the row's 8-element
+// vectors t, t + blockDim.x, ... (VPT of them).
+template <bool F16, bool WF32, int VPT, int MODE>
+__global__ void __launch_bounds__(1024) add_rms_norm_kernel(const NormDev a) {
+  __shared__ uint32_t red[4][32];
+  const int nv = a.N >> 3;
+  uint32_t top = 0;  // max|y| bits of every row this CTA walks (kNormStats)
+  pdl_wait();
+  int turn = 0;
+  for (int64_t row = blockIdx.x; row < a.M; row += gridDim.x, turn ^= 1) {
+    const uint4* xr = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.x) + row * a.ldx);
+    const uint4* rr = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.r) + row * a.ldr);
+    float h[VPT][8];
+    uint4 xv[VPT], rv[VPT];
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) {
+      const int vec = threadIdx.x + j * blockDim.x;
+      xv[j] = rv[j] = make_uint4(0u, 0u, 0u, 0u);
+      if (vec < nv) {
+        xv[j] = __ldg(xr + vec);
+        if (a.r) rv[j] = __ldg(rr + vec);
+      }
+    }
+    float ss = 0.0f;
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) {
+      const int vec = threadIdx.x + j * blockDim.x;
+      unpack8<F16>(xv[j], h[j]);
+      if (a.r) {
+        float rf[8];
+        unpack8<F16>(rv[j], rf);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) h[j][i] += rf[i];
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) ss = fmaf(h[j][i], h[j][i], ss);
+      if (a.h && vec < nv)
+        __stcs(reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.h) + row * a.N) + vec, pack8<F16>(h[j]));
+    }
+    const float sum = __uint_as_float(block_reduce<false>(__float_as_uint(ss), red[turn]));
+    const float rstd = rsqrtf(sum / static_cast<float>(a.N) + a.eps);
+    if (MODE == kNormStats && threadIdx.x == 0) a.rstd[row] = rstd;
+    uint32_t row_top = 0;
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) {
+      const int vec = threadIdx.x + j * blockDim.x;
+      if (vec < nv) {
+        float w[8];
+        load_weight8<F16, WF32>(a.w, vec, w);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          h[j][i] = h[j][i] * rstd * w[i];
+          if (MODE != kNormPlain) row_top = max(row_top, abs_bits(h[j][i]));
+        }
+        if (MODE == kNormPlain)
+          reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.y) + row * a.N)[vec] = pack8<F16>(h[j]);
+      }
+    }
+    if (MODE == kNormRow) {
+      const float s = scale_from_amax_bits(block_reduce<true>(row_top, red[2 + turn]));
+      const float inv = __frcp_rn(s);
+      if (threadIdx.x == 0) a.scale[row] = s;
+#pragma unroll
+      for (int j = 0; j < VPT; ++j) {
+        const int vec = threadIdx.x + j * blockDim.x;
+        if (vec < nv) reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.y) + row * a.N)[vec] = codes8(h[j], inv);
+      }
+    }
+    if (MODE == kNormStats) top = max(top, row_top);
+  }
+  if (MODE == kNormStats) {
+    const uint32_t m = block_reduce<true>(top, red[2]);
+    if (threadIdx.x == 0) a.slots[blockIdx.x] = m;
+  }
+  pdl_trigger();
+}
+
+// The codes of a whole-tensor scale: y is formed again from x, r and the stored 1 / rms
+// in the same order of operations (so max|y| is the value the scale came from).  Rows
+// are walked from the last one up: the rows the first kernel read last are the ones
+// still in L2.
+template <bool F16, bool WF32, int VPT>
+__global__ void __launch_bounds__(1024) rms_norm_codes_kernel(const NormDev a) {
+  __shared__ uint32_t red[32];
+  const int nv = a.N >> 3;
+  pdl_wait();
+  uint32_t m = 0;
+  for (int i = threadIdx.x; i < a.n_slots; i += blockDim.x) m = max(m, __ldcg(a.slots + i));
+  const float s = scale_from_amax_bits(block_reduce<true>(m, red));
+  const float inv = __frcp_rn(s);
+  if (blockIdx.x == 0 && threadIdx.x == 0) *a.scale = s;
+  for (int64_t row = a.M - 1 - blockIdx.x; row >= 0; row -= gridDim.x) {
+    const uint4* xr = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.x) + row * a.ldx);
+    const uint4* rr = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.r) + row * a.ldr);
+    const float rstd = __ldcg(a.rstd + row);
+    uint4 xv[VPT], rv[VPT];
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) {
+      const int vec = threadIdx.x + j * blockDim.x;
+      xv[j] = rv[j] = make_uint4(0u, 0u, 0u, 0u);
+      if (vec < nv) {
+        xv[j] = __ldcs(xr + vec);
+        if (a.r) rv[j] = __ldcs(rr + vec);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) {
+      const int vec = threadIdx.x + j * blockDim.x;
+      if (vec < nv) {
+        float h[8], w[8];
+        unpack8<F16>(xv[j], h);
+        if (a.r) {
+          float rf[8];
+          unpack8<F16>(rv[j], rf);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) h[i] += rf[i];
+        }
+        load_weight8<F16, WF32>(a.w, vec, w);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) h[i] = h[i] * rstd * w[i];
+        __stcs(reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.y) + row * a.N) + vec, codes8(h, inv));
+      }
+    }
+  }
+  pdl_trigger();
+}
+
+struct NormShape {
+  int threads, vpt, ctas;
+};
+// Two vectors a thread (four 16-byte loads in flight) up to 16384 columns, four above;
+// the CTAs that fit 2048 threads an SM.
+static NormShape norm_shape(int64_t M, int64_t N) {
+  const int nv = static_cast<int>(N >> 3);
+  NormShape s;
+  s.vpt = nv <= 64 ? 1 : nv <= 2048 ? 2 : 4;
+  s.threads = ((nv + s.vpt - 1) / s.vpt + 31) / 32 * 32;
+  const int64_t resident = static_cast<int64_t>(sm_count()) * (2048 / s.threads > 12 ? 12 : 2048 / s.threads);
+  const int64_t most = resident < kNormMaxSlots ? resident : kNormMaxSlots;
+  s.ctas = static_cast<int>(M < most ? M : most);
+  return s;
+}
+
+template <bool F16, bool WF32, int VPT>
+static cudaError_t launch_norm(NormDev d, int mode, const NormShape& s, cudaStream_t st) {
+  const dim3 grid(s.ctas), block(s.threads);
+  switch (mode) {
+    case kNormPlain:
+      return launch_kernel(add_rms_norm_kernel<F16, WF32, VPT, kNormPlain>, grid, block, 0, st, true, d);
+    case kNormRow:
+      return launch_kernel(add_rms_norm_kernel<F16, WF32, VPT, kNormRow>, grid, block, 0, st, true, d);
+    default: {
+      d.n_slots = s.ctas;
+      cudaError_t e = launch_kernel(add_rms_norm_kernel<F16, WF32, VPT, kNormStats>, grid, block, 0, st, true, d);
+      if (e != cudaSuccess) return e;
+      return launch_kernel(rms_norm_codes_kernel<F16, WF32, VPT>, grid, block, 0, st, true, d);
+    }
+  }
+}
+template <bool F16, bool WF32>
+static cudaError_t launch_norm_vpt(const NormDev& d, int mode, const NormShape& s, cudaStream_t st) {
+  if (s.vpt == 1) return launch_norm<F16, WF32, 1>(d, mode, s, st);
+  if (s.vpt == 2) return launch_norm<F16, WF32, 2>(d, mode, s, st);
+  return launch_norm<F16, WF32, 4>(d, mode, s, st);
+}
+
+static int norm_entry(const char* who, const void* x, int64_t ldx, const void* r, int64_t ldr, const void* w,
+                      int w_f32, int64_t M, int64_t N, float eps, int f16, void* h, void* y, float* scale, void* ws,
+                      int mode, void* stream) {
+  QIK_REQUIRE(M >= 0 && N > 0 && N % 8 == 0 && N <= 32768, "%s: %lld rows of %lld columns (a multiple of 8, at most 32768)",
+              who, (long long)M, (long long)N);
+  QIK_REQUIRE(eps >= 0.0f, "%s: eps must not be negative", who);
+  if (M == 0) return QIK_OK;
+  QIK_REQUIRE(x && w && y && (mode == kNormPlain || scale) && (mode != kNormStats || ws), "%s: NULL pointer", who);
+  QIK_REQUIRE(aligned16(x) && aligned16(r) && aligned16(w) && aligned16(h) && aligned16(y) && aligned16(ws),
+              "%s: pointers must be 16-byte aligned", who);
+  QIK_REQUIRE(ldx >= N && ldx % 8 == 0 && (!r || (ldr >= N && ldr % 8 == 0)),
+              "%s: row pitches must be multiples of 8 elements and hold a row", who);
+  NormDev d = {};
+  d.x = x, d.r = r, d.w = w, d.h = h, d.y = y, d.scale = scale;
+  d.slots = static_cast<uint32_t*>(ws);
+  d.rstd = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + kNormMaxSlots * sizeof(uint32_t));
+  d.M = M, d.ldx = ldx, d.ldr = ldr, d.N = static_cast<int>(N), d.eps = eps;
+  const NormShape s = norm_shape(M, N);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  QIK_TRY_CUDA(f16 ? (w_f32 ? launch_norm_vpt<true, true>(d, mode, s, st) : launch_norm_vpt<true, false>(d, mode, s, st))
+                   : (w_f32 ? launch_norm_vpt<false, true>(d, mode, s, st)
+                            : launch_norm_vpt<false, false>(d, mode, s, st)));
+  return check_launch(who);
+}
+
+}  // namespace qik
+
+extern "C" size_t qik_add_rms_norm_workspace_bytes(int64_t M) {
+  return qik::kNormMaxSlots * sizeof(uint32_t) + (M > 0 ? static_cast<size_t>(M) * sizeof(float) : 0);
+}
+
+extern "C" int qik_add_rms_norm(const void* x, int64_t ldx, const void* residual, int64_t ldr, const void* weight,
+                                int weight_f32, int64_t M, int64_t N, float eps, int f16, void* sum_out, void* out,
+                                void* stream) {
+  return qik::norm_entry("qik_add_rms_norm", x, ldx, residual, ldr, weight, weight_f32, M, N, eps, f16, sum_out, out,
+                         nullptr, nullptr, qik::kNormPlain, stream);
+}
+
+extern "C" int qik_add_rms_norm_e4m3(const void* x, int64_t ldx, const void* residual, int64_t ldr, const void* weight,
+                                     int weight_f32, int64_t M, int64_t N, float eps, int f16, void* sum_out, void* q,
+                                     float* scale, int row_scales, void* ws, void* stream) {
+  return qik::norm_entry("qik_add_rms_norm_e4m3", x, ldx, residual, ldr, weight, weight_f32, M, N, eps, f16, sum_out,
+                         q, scale, ws, row_scales ? qik::kNormRow : qik::kNormStats, stream);
+}

@@ -20,7 +20,9 @@ EPI_SCALE, EPI_GELU_TANH, EPI_SCATTER, EPI_SWIGLU = 0, 1, 2, 3
 GEMM_TILE_AUTO, GEMM_TILE_PAIR_256, GEMM_TILE_SINGLE_256, GEMM_TILE_SINGLE_128, GEMM_TILE_SINGLE_64, GEMM_TILE_SWAP_16 = range(6)
 TP_MAX_WORLD = 8
 ATTN_HAS_CACHE, ATTN_HAS_KEY_VALID, ATTN_UNIFORM, ATTN_V_FP8, ATTN_F16 = 1, 2, 4, 8, 16
-STATUS_OK, STATUS_TIMEOUT = 0, 1
+ROTARY_INTERLEAVED, ROTARY_F16, ROTARY_PAGED, ROTARY_POS64, ROTARY_SLOT64 = 1, 2, 4, 8, 16
+PAGED_CAUSAL, PAGED_F16 = 1, 2
+STATUS_OK, STATUS_TIMEOUT, STATUS_BAD_INDEX = 0, 1, 2
 
 _i64, _i32, _f32, _vp, _u64 = ctypes.c_int64, ctypes.c_int, ctypes.c_float, ctypes.c_void_p, ctypes.c_uint64
 
@@ -41,6 +43,42 @@ class AttnArgs(ctypes.Structure):
         ("sm_scale", _f32),
         ("flags", _i32),
         ("amax_out", _vp),
+    ]
+
+
+class RotaryArgs(ctypes.Structure):
+    """Mirror of ``qik_rotary_args`` (include/qik.h)."""
+    _fields_ = [
+        ("q", _vp), ("k", _vp), ("v", _vp), ("q_out", _vp), ("k_out", _vp), ("v_out", _vp),
+        ("positions", _vp), ("slots", _vp), ("cos", _vp), ("sin", _vp),
+        ("T", _i64), ("HQ", _i64), ("HK", _i64), ("D", _i64), ("rot", _i64), ("P", _i64),
+        ("q_st", _i64), ("q_sh", _i64), ("k_st", _i64), ("k_sh", _i64), ("v_st", _i64), ("v_sh", _i64),
+        ("page", _i64), ("pages", _i64),
+        ("kp_s0", _i64), ("kp_sh", _i64), ("kp_ss", _i64), ("vp_s0", _i64), ("vp_sh", _i64), ("vp_ss", _i64),
+        ("flags", _i32),
+    ]
+
+
+class PagePools(ctypes.Structure):
+    """Mirror of ``qik_page_pools`` (include/qik.h)."""
+    _fields_ = [
+        ("k", _vp), ("v", _vp),
+        ("layers", _i64), ("pages", _i64), ("heads", _i64), ("page", _i64), ("token_bytes", _i64),
+        ("k_layer_bytes", _i64), ("k_page_bytes", _i64), ("k_head_bytes", _i64),
+        ("v_layer_bytes", _i64), ("v_page_bytes", _i64), ("v_head_bytes", _i64),
+    ]
+
+
+class PagedAttnArgs(ctypes.Structure):
+    """Mirror of ``qik_paged_attn_args`` (include/qik.h)."""
+    _fields_ = [
+        ("q", _vp), ("k_pages", _vp), ("v_pages", _vp), ("out", _vp),
+        ("page_table", _vp), ("seq_lens", _vp), ("query_starts", _vp),
+        ("B", _i64), ("T", _i64), ("HQ", _i64), ("HK", _i64), ("D", _i64), ("W", _i64), ("pages", _i64), ("page", _i64),
+        ("max_new", _i64), ("max_kv", _i64),
+        ("q_st", _i64), ("q_sh", _i64), ("o_st", _i64), ("o_sh", _i64), ("table_st", _i64),
+        ("kp_s0", _i64), ("kp_sh", _i64), ("kp_ss", _i64), ("vp_s0", _i64), ("vp_sh", _i64), ("vp_ss", _i64),
+        ("sm_scale", _f32), ("window", _i32), ("sinks", _i32), ("flags", _i32),
     ]
 
 
@@ -82,6 +120,14 @@ SIGNATURES = {
                                             _vp, _vp, _vp]),
     "qik_gate_residual": (_i32, [_vp, _vp, _i64, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _vp, _vp]),
     "qik_swiglu": (_i32, [_vp, _i64, _vp, _i64, _i64, _i64, _vp, _i64, _vp, _vp]),
+    "qik_add_rms_norm": (_i32, [_vp, _i64, _vp, _i64, _vp, _i32, _i64, _i64, _f32, _i32, _vp, _vp, _vp]),
+    "qik_add_rms_norm_workspace_bytes": (ctypes.c_size_t, [_i64]),
+    "qik_add_rms_norm_e4m3": (_i32, [_vp, _i64, _vp, _i64, _vp, _i32, _i64, _i64, _f32, _i32, _vp, _vp, _vp, _i32,
+                                     _vp, _vp]),
+    "qik_rotary": (_i32, [ctypes.POINTER(RotaryArgs), _vp, _vp]),
+    "qik_copy_pages": (_i32, [ctypes.POINTER(PagePools), _vp, _i64, _vp]),
+    "qik_paged_attention_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(PagedAttnArgs)]),
+    "qik_paged_attention": (_i32, [ctypes.POINTER(PagedAttnArgs), _vp, ctypes.c_size_t, _vp, _vp]),
     "qik_selftest_wait_timeout": (_i32, [_vp, _u64, _vp]),
     "qik_ipc_handle_bytes": (ctypes.c_size_t, []),
     "qik_ipc_export": (_i32, [_vp, _vp, ctypes.POINTER(_u64)]),
@@ -140,6 +186,30 @@ def check(rc: int, what: str) -> None:
 
 def stream_ptr(device: torch.device | None = None) -> int:
     return torch.cuda.current_stream(device).cuda_stream
+
+
+def on_device(name: str, device: torch.device, *args):
+    """What the entry point ``name`` returns for ``args`` with ``device`` current (its answer
+    may depend on that device's SMs)."""
+    fn = getattr(_lib if _lib is not None else load(), name)
+    if torch.cuda.current_device() == device.index:
+        return fn(*args)
+    with torch.cuda.device(device):
+        return fn(*args)
+
+
+def launch(name: str, device: torch.device, *args) -> None:
+    """Call the entry point ``name`` with ``args`` and the current stream of ``device``,
+    with that device current (its tensors need not be on the current one)."""
+    fn = getattr(_lib if _lib is not None else load(), name)
+    idx = device.index
+    if torch.cuda.current_device() == idx:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(idx))
+    else:
+        with torch.cuda.device(idx):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(idx))
+    if rc != QIK_OK:
+        check(rc, name)
 
 
 def ptr(t: torch.Tensor | None) -> int | None:
