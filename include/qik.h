@@ -491,11 +491,11 @@ int qik_add_rms_norm(const void* x, int64_t ldx, const void* residual, int64_t l
  * (row_scales != 0: scale [M]) or over the whole tensor (scale [1], the dynamic scale
  * that qik_fp8_gemm takes), q [M, N] = e4m3 (nearest even) of y / scale.  y is not
  * rounded to 16 bits in between; NaN in a row reaches its scale.
- *   ws: qik_add_rms_norm_workspace_bytes(M) bytes, 16-byte aligned, not initialised by
- *   the caller (whole-tensor scale only; NULL for row scales).  The whole-tensor form
+ *   ws: qik_add_rms_norm_workspace_bytes(M, N) bytes, 16-byte aligned, not initialised by
+ *   the caller (whole-tensor scale only; NULL for row scales and where it is 0 bytes).  The whole-tensor form
  *   reads x and residual twice: sum_out must not overlap them.
  */
-size_t qik_add_rms_norm_workspace_bytes(int64_t M);
+size_t qik_add_rms_norm_workspace_bytes(int64_t M, int64_t N);
 int qik_add_rms_norm_e4m3(const void* x, int64_t ldx, const void* residual, int64_t ldr, const void* weight,
                           int weight_f32, int64_t M, int64_t N, float eps, int f16, void* sum_out, void* q,
                           float* scale, int row_scales, void* ws, void* stream);

@@ -230,6 +230,92 @@ __global__ void __launch_bounds__(1024) rms_norm_codes_kernel(const NormDev a) {
   pdl_trigger();
 }
 
+// Few rows (at most two for each CTA of one 8-CTA cluster) with a whole-tensor scale: the
+// rows stay in registers while the CTAs exchange their max|y| through distributed shared
+// memory, so one launch without a workspace does it.  Three rows of 4096: one launch and
+// one allocation less on the host than the two kernels (which these sizes are bound by).
+constexpr int kNormCluster = 8;
+constexpr int kNormClusterRows = 2;
+template <bool F16, bool WF32, int VPT>
+__global__ void __launch_bounds__(1024) __cluster_dims__(kNormCluster, 1, 1) add_rms_norm_few_kernel(const NormDev a) {
+  __shared__ uint32_t red[3][32];
+  __shared__ uint32_t tops[kNormCluster];  // every CTA's max|y| bits, written by their owners
+  const int nv = a.N >> 3;
+  const uint32_t rank = cluster_ctarank();
+  pdl_wait();
+  float h[kNormClusterRows][VPT][8];
+  uint4 xv[kNormClusterRows][VPT], rv[kNormClusterRows][VPT];
+#pragma unroll
+  for (int k = 0; k < kNormClusterRows; ++k) {
+    const int64_t row = rank + k * kNormCluster;
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) {
+      const int vec = threadIdx.x + j * blockDim.x;
+      xv[k][j] = rv[k][j] = make_uint4(0u, 0u, 0u, 0u);
+      if (row < a.M && vec < nv) {
+        xv[k][j] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.x) + row * a.ldx) + vec);
+        if (a.r) rv[k][j] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.r) + row * a.ldr) + vec);
+      }
+    }
+  }
+  uint32_t top = 0;
+#pragma unroll
+  for (int k = 0; k < kNormClusterRows; ++k) {
+    const int64_t row = rank + k * kNormCluster;
+    float ss = 0.0f;
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) {
+      const int vec = threadIdx.x + j * blockDim.x;
+      unpack8<F16>(xv[k][j], h[k][j]);
+      if (a.r) {
+        float rf[8];
+        unpack8<F16>(rv[k][j], rf);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) h[k][j][i] += rf[i];
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) ss = fmaf(h[k][j][i], h[k][j][i], ss);
+      if (a.h && row < a.M && vec < nv)
+        reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.h) + row * a.N)[vec] = pack8<F16>(h[k][j]);
+    }
+    const float sum = __uint_as_float(block_reduce<false>(__float_as_uint(ss), red[k]));
+    const float rstd = rsqrtf(sum / static_cast<float>(a.N) + a.eps);
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) {
+      const int vec = threadIdx.x + j * blockDim.x;
+      if (row < a.M && vec < nv) {
+        float w[8];
+        load_weight8<F16, WF32>(a.w, vec, w);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          h[k][j][i] = h[k][j][i] * rstd * w[i];
+          top = max(top, abs_bits(h[k][j][i]));
+        }
+      }
+    }
+  }
+  top = block_reduce<true>(top, red[kNormClusterRows]);
+  if (threadIdx.x < kNormCluster) st_cluster_u32(mapa_shared(&tops[rank], threadIdx.x), top);
+  cluster_sync();
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < kNormCluster; ++i) m = max(m, tops[i]);
+  const float s = scale_from_amax_bits(m);
+  const float inv = __frcp_rn(s);
+  if (rank == 0 && threadIdx.x == 0) *a.scale = s;
+#pragma unroll
+  for (int k = 0; k < kNormClusterRows; ++k) {
+    const int64_t row = rank + k * kNormCluster;
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) {
+      const int vec = threadIdx.x + j * blockDim.x;
+      if (row < a.M && vec < nv)
+        reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.y) + row * a.N)[vec] = codes8(h[k][j], inv);
+    }
+  }
+  pdl_trigger();
+}
+
 struct NormShape {
   int threads, vpt, ctas;
 };
@@ -255,6 +341,8 @@ static cudaError_t launch_norm(NormDev d, int mode, const NormShape& s, cudaStre
     case kNormRow:
       return launch_kernel(add_rms_norm_kernel<F16, WF32, VPT, kNormRow>, grid, block, 0, st, true, d);
     default: {
+      if (VPT <= 2 && d.M <= kNormCluster * kNormClusterRows)
+        return launch_kernel(add_rms_norm_few_kernel<F16, WF32, VPT <= 2 ? VPT : 2>, dim3(kNormCluster), block, 0, st, true, d);
       d.n_slots = s.ctas;
       cudaError_t e = launch_kernel(add_rms_norm_kernel<F16, WF32, VPT, kNormStats>, grid, block, 0, st, true, d);
       if (e != cudaSuccess) return e;
@@ -276,7 +364,8 @@ static int norm_entry(const char* who, const void* x, int64_t ldx, const void* r
               who, (long long)M, (long long)N);
   QIK_REQUIRE(eps >= 0.0f, "%s: eps must not be negative", who);
   if (M == 0) return QIK_OK;
-  QIK_REQUIRE(x && w && y && (mode == kNormPlain || scale) && (mode != kNormStats || ws), "%s: NULL pointer", who);
+  QIK_REQUIRE(x && w && y && (mode == kNormPlain || scale) && (mode != kNormStats || ws || M <= kNormCluster * kNormClusterRows && N <= 16384),
+              "%s: NULL pointer", who);
   QIK_REQUIRE(aligned16(x) && aligned16(r) && aligned16(w) && aligned16(h) && aligned16(y) && aligned16(ws),
               "%s: pointers must be 16-byte aligned", who);
   QIK_REQUIRE(ldx >= N && ldx % 8 == 0 && (!r || (ldr >= N && ldr % 8 == 0)),
@@ -296,8 +385,9 @@ static int norm_entry(const char* who, const void* x, int64_t ldx, const void* r
 
 }  // namespace qik
 
-extern "C" size_t qik_add_rms_norm_workspace_bytes(int64_t M) {
-  return qik::kNormMaxSlots * sizeof(uint32_t) + (M > 0 ? static_cast<size_t>(M) * sizeof(float) : 0);
+extern "C" size_t qik_add_rms_norm_workspace_bytes(int64_t M, int64_t N) {
+  if (M <= qik::kNormCluster * qik::kNormClusterRows && N <= 16384) return 0;
+  return qik::kNormMaxSlots * sizeof(uint32_t) + static_cast<size_t>(M) * sizeof(float);
 }
 
 extern "C" int qik_add_rms_norm(const void* x, int64_t ldx, const void* residual, int64_t ldr, const void* weight,

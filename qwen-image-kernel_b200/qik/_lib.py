@@ -7,6 +7,7 @@ raises instead of computing anything elsewhere.
 from __future__ import annotations
 
 import ctypes
+import struct
 import threading
 from pathlib import Path
 
@@ -46,40 +47,18 @@ class AttnArgs(ctypes.Structure):
     ]
 
 
-class RotaryArgs(ctypes.Structure):
-    """Mirror of ``qik_rotary_args`` (include/qik.h)."""
-    _fields_ = [
-        ("q", _vp), ("k", _vp), ("v", _vp), ("q_out", _vp), ("k_out", _vp), ("v_out", _vp),
-        ("positions", _vp), ("slots", _vp), ("cos", _vp), ("sin", _vp),
-        ("T", _i64), ("HQ", _i64), ("HK", _i64), ("D", _i64), ("rot", _i64), ("P", _i64),
-        ("q_st", _i64), ("q_sh", _i64), ("k_st", _i64), ("k_sh", _i64), ("v_st", _i64), ("v_sh", _i64),
-        ("page", _i64), ("pages", _i64),
-        ("kp_s0", _i64), ("kp_sh", _i64), ("kp_ss", _i64), ("vp_s0", _i64), ("vp_sh", _i64), ("vp_ss", _i64),
-        ("flags", _i32),
-    ]
-
-
-class PagePools(ctypes.Structure):
-    """Mirror of ``qik_page_pools`` (include/qik.h)."""
-    _fields_ = [
-        ("k", _vp), ("v", _vp),
-        ("layers", _i64), ("pages", _i64), ("heads", _i64), ("page", _i64), ("token_bytes", _i64),
-        ("k_layer_bytes", _i64), ("k_page_bytes", _i64), ("k_head_bytes", _i64),
-        ("v_layer_bytes", _i64), ("v_page_bytes", _i64), ("v_head_bytes", _i64),
-    ]
-
-
-class PagedAttnArgs(ctypes.Structure):
-    """Mirror of ``qik_paged_attn_args`` (include/qik.h)."""
-    _fields_ = [
-        ("q", _vp), ("k_pages", _vp), ("v_pages", _vp), ("out", _vp),
-        ("page_table", _vp), ("seq_lens", _vp), ("query_starts", _vp),
-        ("B", _i64), ("T", _i64), ("HQ", _i64), ("HK", _i64), ("D", _i64), ("W", _i64), ("pages", _i64), ("page", _i64),
-        ("max_new", _i64), ("max_kv", _i64),
-        ("q_st", _i64), ("q_sh", _i64), ("o_st", _i64), ("o_sh", _i64), ("table_st", _i64),
-        ("kp_s0", _i64), ("kp_sh", _i64), ("kp_ss", _i64), ("vp_s0", _i64), ("vp_sh", _i64), ("vp_ss", _i64),
-        ("sm_scale", _f32), ("window", _i32), ("sinks", _i32), ("flags", _i32),
-    ]
+# The structs of the calls that a decoder makes in every layer, as packers: one call packs
+# the fields in the order of include/qik.h (native alignment), several times faster than a
+# ctypes.Structure; the bytes are passed where the entry point takes a pointer.
+# qik_rotary_args: q k v q_out k_out v_out positions slots cos sin | T HQ HK D rot P |
+#   q_st q_sh k_st k_sh v_st v_sh | page pages | kp_s0 kp_sh kp_ss vp_s0 vp_sh vp_ss | flags
+pack_rotary = struct.Struct("@10P20qi0q").pack
+# qik_page_pools: k v | layers pages heads page token_bytes | k layer, page, head bytes | v ...
+pack_pools = struct.Struct("@2P11q").pack
+# qik_paged_attn_args: q k_pages v_pages out page_table seq_lens query_starts | B T HQ HK D W
+#   pages page max_new max_kv | q_st q_sh o_st o_sh table_st | kp_s0 kp_sh kp_ss vp_s0 vp_sh vp_ss |
+#   sm_scale | window sinks flags
+pack_paged_attn = struct.Struct("@7P21qf3i0q").pack
 
 
 # name -> (restype, argtypes)
@@ -121,13 +100,13 @@ SIGNATURES = {
     "qik_gate_residual": (_i32, [_vp, _vp, _i64, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _vp, _vp]),
     "qik_swiglu": (_i32, [_vp, _i64, _vp, _i64, _i64, _i64, _vp, _i64, _vp, _vp]),
     "qik_add_rms_norm": (_i32, [_vp, _i64, _vp, _i64, _vp, _i32, _i64, _i64, _f32, _i32, _vp, _vp, _vp]),
-    "qik_add_rms_norm_workspace_bytes": (ctypes.c_size_t, [_i64]),
+    "qik_add_rms_norm_workspace_bytes": (ctypes.c_size_t, [_i64, _i64]),
     "qik_add_rms_norm_e4m3": (_i32, [_vp, _i64, _vp, _i64, _vp, _i32, _i64, _i64, _f32, _i32, _vp, _vp, _vp, _i32,
                                      _vp, _vp]),
-    "qik_rotary": (_i32, [ctypes.POINTER(RotaryArgs), _vp, _vp]),
-    "qik_copy_pages": (_i32, [ctypes.POINTER(PagePools), _vp, _i64, _vp]),
-    "qik_paged_attention_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(PagedAttnArgs)]),
-    "qik_paged_attention": (_i32, [ctypes.POINTER(PagedAttnArgs), _vp, ctypes.c_size_t, _vp, _vp]),
+    "qik_rotary": (_i32, [_vp, _vp, _vp]),
+    "qik_copy_pages": (_i32, [_vp, _vp, _i64, _vp]),
+    "qik_paged_attention_workspace_bytes": (ctypes.c_size_t, [_vp]),
+    "qik_paged_attention": (_i32, [_vp, _vp, ctypes.c_size_t, _vp, _vp]),
     "qik_selftest_wait_timeout": (_i32, [_vp, _u64, _vp]),
     "qik_ipc_handle_bytes": (ctypes.c_size_t, []),
     "qik_ipc_export": (_i32, [_vp, _vp, ctypes.POINTER(_u64)]),
@@ -188,22 +167,21 @@ def stream_ptr(device: torch.device | None = None) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
-def on_device(name: str, device: torch.device, *args):
-    """What the entry point ``name`` returns for ``args`` with ``device`` current (its answer
+def on_device(name: str, idx: int, *args):
+    """What the entry point ``name`` returns for ``args`` with device ``idx`` current (its answer
     may depend on that device's SMs)."""
-    fn = getattr(_lib if _lib is not None else load(), name)
-    if torch.cuda.current_device() == device.index:
+    fn = getattr(_lib or load(), name)
+    if torch._C._cuda_getDevice() == idx:
         return fn(*args)
-    with torch.cuda.device(device):
+    with torch.cuda.device(idx):
         return fn(*args)
 
 
-def launch(name: str, device: torch.device, *args) -> None:
-    """Call the entry point ``name`` with ``args`` and the current stream of ``device``,
-    with that device current (its tensors need not be on the current one)."""
-    fn = getattr(_lib if _lib is not None else load(), name)
-    idx = device.index
-    if torch.cuda.current_device() == idx:
+def launch(name: str, idx: int, *args) -> None:
+    """Call the entry point ``name`` with ``args`` and the current stream of device ``idx``, with
+    that device current (its tensors need not be on the current one)."""
+    fn = getattr(_lib or load(), name)
+    if torch._C._cuda_getDevice() == idx:
         rc = fn(*args, torch._C._cuda_getCurrentRawStream(idx))
     else:
         with torch.cuda.device(idx):
@@ -217,6 +195,7 @@ def ptr(t: torch.Tensor | None) -> int | None:
 
 
 _status: dict[int, torch.Tensor] = {}
+_status_ptr: dict[int, int] = {}
 
 
 def status_word(device: torch.device) -> torch.Tensor:
@@ -227,6 +206,14 @@ def status_word(device: torch.device) -> torch.Tensor:
         t = torch.zeros(4, dtype=torch.int32, device=torch.device("cuda", idx))
         _status[idx] = t
     return t
+
+
+def status_ptr(idx: int) -> int:
+    """Address of device ``idx``'s status word."""
+    p = _status_ptr.get(idx)
+    if p is None:
+        p = _status_ptr[idx] = status_word(torch.device("cuda", idx)).data_ptr()
+    return p
 
 
 def device_status(device: torch.device | None = None) -> int:

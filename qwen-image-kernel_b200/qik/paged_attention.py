@@ -8,8 +8,6 @@ all of it, or the last ``window`` keys and the first ``sinks``.  The kernels
 """
 from __future__ import annotations
 
-import ctypes
-
 import torch
 
 from . import _lib as L
@@ -43,26 +41,26 @@ def paged_attention(
     behind query_starts[B] are not written.  No sequence may bring more than ``max_new``
     tokens; ``max_kv`` only chooses launch shapes.  Lengths, starts and page numbers outside
     their tensors are skipped and set ``STATUS_BAD_INDEX`` (``qik._lib.device_status``)."""
-    dev = q.device
     if not q.is_cuda:
         raise ValueError("qik: q must be a CUDA tensor (the kernels have no CPU path)")
-    if q.dtype not in _TYPES:
-        raise TypeError(f"qik: paged_attention: bf16 or fp16, got {q.dtype}")
+    dev, dtype = q.device, q.dtype
+    if dtype not in _TYPES:
+        raise TypeError(f"qik: paged_attention: bf16 or fp16, got {dtype}")
     if q.dim() != 3 or q.shape[2] not in (64, 128):
         raise ValueError(f"qik: q is {tuple(q.shape)}: expected [tokens, heads, 64 or 128]")
     T, HQ, D = q.shape
-    check_pages(k_pages, v_pages, q)
-    pages, HK, page, _ = k_pages.shape
+    pages, HK, page, strides = check_pages(k_pages, v_pages, D, dtype, dev)
     if HQ == 0 or HQ % HK:
         raise ValueError(f"qik: {HQ} query heads do not share {HK} key heads evenly")
-    B = seq_lens.shape[0]
-    for name, t, dim in (("page_table", page_table, 2), ("seq_lens", seq_lens, 1), ("query_starts", query_starts, 1)):
-        if t.dtype != torch.int32 or t.device != dev or t.dim() != dim:
-            raise ValueError(f"qik: {name} is {tuple(t.shape)} {t.dtype} on {t.device}: expected int32 on {dev}")
-    if page_table.shape[0] != B or query_starts.shape[0] != B + 1:
+    i32 = torch.int32
+    if page_table.dtype != i32 or seq_lens.dtype != i32 or query_starts.dtype != i32 or page_table.device != dev or \
+            seq_lens.device != dev or query_starts.device != dev:
+        raise ValueError(f"qik: page_table, seq_lens and query_starts must be int32 on {dev}")
+    if page_table.dim() != 2 or seq_lens.dim() != 1 or query_starts.dim() != 1 or \
+            page_table.shape[0] != seq_lens.shape[0] or query_starts.shape[0] != seq_lens.shape[0] + 1:
         raise ValueError(f"qik: page_table {tuple(page_table.shape)}, seq_lens {tuple(seq_lens.shape)} and query_starts "
-                         f"{tuple(query_starts.shape)} are not of one batch")
-    W = page_table.shape[1]
+                         f"{tuple(query_starts.shape)}: expected [B, W], [B] and [B + 1]")
+    B, W = page_table.shape
     if not 0 <= max_new <= T:
         raise ValueError(f"qik: max_new is {max_new}, q has {T} tokens")
     if max_kv is None:
@@ -73,35 +71,32 @@ def paged_attention(
         sm_scale = D ** -0.5
     elif not 0.0 < sm_scale < 1e30:
         raise ValueError(f"qik: sm_scale must be positive and finite, got {sm_scale}")
-    st, sh, sd = q.stride()
-    if sd != 1 or st % 8 or sh % 8 or q.data_ptr() % 16:
+    q_st, q_sh, sd = q.stride()
+    if sd != 1 or (q_st | q_sh) % 8 or q.data_ptr() % 16:
         q = q.clone(memory_format=torch.contiguous_format)
-        st, sh, _ = q.stride()
+        q_st, q_sh, _ = q.stride()
     if out is None:
-        out = torch.empty((T, HQ, D), dtype=q.dtype, device=dev)
-        o_st, o_sh = HQ * D, D
-    else:
-        if out.shape != q.shape or out.dtype != q.dtype or out.device != dev:
-            raise ValueError(f"qik: out is {tuple(out.shape)} {out.dtype} on {out.device}: expected {tuple(q.shape)} {q.dtype}")
-        o_st, o_sh, sd = out.stride()
-        if sd != 1 or o_st % 8 or o_sh % 8 or out.data_ptr() % 16:
-            raise ValueError("qik: out needs a unit column stride, strides of 16 bytes and 16-byte alignment")
-    if page_table.stride(1) != 1 and W > 1:
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    elif out.shape != q.shape or out.dtype != dtype or out.device != dev:
+        raise ValueError(f"qik: out is {tuple(out.shape)} {out.dtype} on {out.device}: expected {tuple(q.shape)} {dtype}")
+    o_st, o_sh, sd = out.stride()
+    if sd != 1 or (o_st | o_sh) % 8 or out.data_ptr() % 16:
+        raise ValueError("qik: out needs a unit column stride, strides of 16 bytes and 16-byte alignment")
+    t_st, td = page_table.stride()
+    if td != 1 and W > 1:
         page_table = page_table.contiguous()
+        t_st = W
     if not seq_lens.is_contiguous():
         seq_lens = seq_lens.contiguous()
     if not query_starts.is_contiguous():
         query_starts = query_starts.contiguous()
-    k0, kh, ks, _ = k_pages.stride()
-    v0, vh, vs, _ = v_pages.stride()
-    a = L.PagedAttnArgs(q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(), page_table.data_ptr(),
-                        seq_lens.data_ptr(), query_starts.data_ptr(), B, T, HQ, HK, D, W, pages, page, max_new, max_kv,
-                        st, sh, o_st, o_sh, page_table.stride(0), k0, kh, ks, v0, vh, vs, sm_scale, window, sinks,
-                        (L.PAGED_CAUSAL if causal else 0) | (L.PAGED_F16 if q.dtype == torch.float16 else 0))
-    ref = ctypes.byref(a)
-    # the workspace is the caller's stream's: torch hands its memory on only to later work there
-    with_ws = L.on_device("qik_paged_attention_workspace_bytes", dev, ref)
-    ws = torch.empty(with_ws, dtype=torch.uint8, device=dev) if with_ws else None
-    L.launch("qik_paged_attention", dev, ref, None if ws is None else ws.data_ptr(), with_ws,
-             L.status_word(dev).data_ptr())
+    args = L.pack_paged_attn(q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(), page_table.data_ptr(),
+                             seq_lens.data_ptr(), query_starts.data_ptr(), B, T, HQ, HK, D, W, pages, page, max_new, max_kv,
+                             q_st, q_sh, o_st, o_sh, t_st, *strides, sm_scale, window, sinks,
+                             (L.PAGED_CAUSAL if causal else 0) | (L.PAGED_F16 if dtype == torch.float16 else 0))
+    idx = dev.index
+    # a workspace of this call alone: torch hands its memory on only to later work of the stream
+    n = L.on_device("qik_paged_attention_workspace_bytes", idx, args)
+    ws = q.new_empty(n, dtype=torch.uint8) if n else None
+    L.launch("qik_paged_attention", idx, args, None if ws is None else ws.data_ptr(), n, L.status_ptr(idx))
     return out

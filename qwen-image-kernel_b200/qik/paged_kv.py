@@ -11,7 +11,6 @@ pages and copies the rest of the last one, so that a store never writes to a sha
 """
 from __future__ import annotations
 
-import ctypes
 import heapq
 
 import numpy as np
@@ -46,24 +45,22 @@ def copy_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, moves) -> None:
         return
     if wide.ndim != 2 or wide.shape[1] != 3 or wide.dtype.kind not in "iu":
         raise ValueError("qik: moves is a sequence of (from, to, tokens)")
-    m = np.ascontiguousarray(wide, dtype=np.int32)
-    if wide.dtype != np.int32 and (m != wide).any():
-        raise ValueError("qik: a move is outside 32 bits")
-    size = k_pages.element_size()
-    k_strides, v_strides = k_pages.stride(), v_pages.stride()
-    layers = 1
-    if k_pages.dim() == 5:
-        layers = k_pages.shape[0]
+    if wide.dtype == np.int32 and wide.flags.c_contiguous:
+        m = wide
     else:
-        k_strides, v_strides = (0, *k_strides), (0, *v_strides)
-    pages, heads, page, D = k_pages.shape[-4:]
-    for s in (k_strides, v_strides):
-        if s[4] != 1 or s[3] != D or min(s) < 0:
-            raise ValueError("qik: a head's tokens must be contiguous in a page")
-    p = L.PagePools(k_pages.data_ptr(), v_pages.data_ptr(), layers, pages, heads, page, D * size,
-                    k_strides[0] * size, k_strides[1] * size, k_strides[2] * size,
-                    v_strides[0] * size, v_strides[1] * size, v_strides[2] * size)
-    L.launch("qik_copy_pages", k_pages.device, ctypes.byref(p), m.ctypes.data, m.shape[0])
+        if wide.max() > 0x7FFFFFFF or wide.min() < 0:
+            raise ValueError("qik: copy_pages: a move is outside the pool")
+        m = wide.astype(np.int32, order="C")
+    size = k_pages.element_size()
+    shape, ks, vs = k_pages.shape, k_pages.stride(), v_pages.stride()
+    if len(shape) == 4:
+        shape, ks, vs = (1, *shape), (0, *ks), (0, *vs)
+    layers, pages, heads, page, D = shape
+    if ks[4] != 1 or vs[4] != 1 or ks[3] != D or vs[3] != D:
+        raise ValueError("qik: a head's tokens must be contiguous in a page")
+    L.launch("qik_copy_pages", k_pages.device.index,
+             L.pack_pools(k_pages.data_ptr(), v_pages.data_ptr(), layers, pages, heads, page, D * size, ks[0] * size,
+                          ks[1] * size, ks[2] * size, vs[0] * size, vs[1] * size, vs[2] * size), m.ctypes.data, len(m))
 
 
 class PagedStep:

@@ -20,42 +20,47 @@ from . import _lib as L
 _TYPES = (torch.bfloat16, torch.float16)
 
 
-def _row_pitch(t: torch.Tensor, M: int, N: int) -> tuple[torch.Tensor, int]:
+_one: dict = {}  # a scale's shape and type on each device, for empty_like
+
+
+def _row_pitch(t: torch.Tensor, N: int) -> tuple[torch.Tensor, int]:
     """t ([..., N]) and its row pitch in elements, copied only where the leading dims do
     not flatten to rows of one pitch or the alignment is not 16 bytes."""
     if t.is_contiguous():
-        if t.data_ptr() % 16 == 0:
-            return t, N
-        return t.clone(), N
+        return (t, N) if t.data_ptr() % 16 == 0 else (t.clone(), N)
     if t.dim() == 2 and t.stride(1) == 1 and t.stride(0) >= N and t.stride(0) % 8 == 0 and t.data_ptr() % 16 == 0:
         return t, t.stride(0)
     return t.contiguous(), N
 
 
-def _check(x: torch.Tensor, residual: torch.Tensor | None, weight: torch.Tensor, who: str) -> tuple[int, int]:
+def _prepare(x: torch.Tensor, residual: torch.Tensor | None, weight: torch.Tensor, who: str) -> tuple:
+    """(x, its pitch, the residual's address and pitch, weight, whether it is fp32, rows,
+    columns), checked; and the tensors that have to live until the launch."""
     if not x.is_cuda:
         raise ValueError(f"qik: {who}: x must be a CUDA tensor (the kernels have no CPU path)")
-    if x.dtype not in _TYPES:
-        raise TypeError(f"qik: {who}: bf16 or fp16, got {x.dtype}")
-    if x.dim() == 0:
+    dtype, shape, dev = x.dtype, x.shape, x.device
+    if dtype not in _TYPES:
+        raise TypeError(f"qik: {who}: bf16 or fp16, got {dtype}")
+    if not shape:
         raise ValueError(f"qik: {who}: x needs at least one dimension")
-    N = x.shape[-1]
-    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype or residual.device != x.device):
-        raise ValueError(f"qik: {who}: residual {tuple(residual.shape)} {residual.dtype} on {residual.device} does not "
-                         f"match x {tuple(x.shape)} {x.dtype} on {x.device}")
-    if weight.dim() != 1 or weight.shape[0] != N or weight.device != x.device:
-        raise ValueError(f"qik: {who}: weight has shape {tuple(weight.shape)} on {weight.device}, expected ({N},) on "
-                         f"{x.device}")
-    if weight.dtype != x.dtype and weight.dtype != torch.float32:
-        raise TypeError(f"qik: {who}: weight must be {x.dtype} or fp32, got {weight.dtype}")
+    N = shape[-1]
     if N == 0 or N % 8 or N > 32768:
         raise ValueError(f"qik: {who}: {N} columns (a multiple of 8, at most 32768)")
-    return x.numel() // N, N
-
-
-def _weight(weight: torch.Tensor) -> torch.Tensor:
-    return weight if weight.stride(0) == 1 and weight.data_ptr() % 16 == 0 else weight.clone(
-        memory_format=torch.contiguous_format)
+    if weight.shape != (N,) or weight.device != dev:
+        raise ValueError(f"qik: {who}: weight has shape {tuple(weight.shape)} on {weight.device}, expected ({N},) on {dev}")
+    f32 = weight.dtype == torch.float32
+    if not f32 and weight.dtype != dtype:
+        raise TypeError(f"qik: {who}: weight must be {dtype} or fp32, got {weight.dtype}")
+    if not weight.is_contiguous() or weight.data_ptr() % 16:
+        weight = weight.clone(memory_format=torch.contiguous_format)
+    x, ldx = _row_pitch(x, N)
+    if residual is None:
+        return x, ldx, None, 0, weight, f32, x.numel() // N, N, None
+    if residual.shape != shape or residual.dtype != dtype or residual.device != dev:
+        raise ValueError(f"qik: {who}: residual {tuple(residual.shape)} {residual.dtype} on {residual.device} does not "
+                         f"match x {tuple(shape)} {dtype} on {dev}")
+    residual, ldr = _row_pitch(residual, N)
+    return x, ldx, residual.data_ptr(), ldr, weight, f32, x.numel() // N, N, residual
 
 
 def fused_add_rms_norm(x: torch.Tensor, residual: torch.Tensor | None, weight: torch.Tensor,
@@ -63,17 +68,12 @@ def fused_add_rms_norm(x: torch.Tensor, residual: torch.Tensor | None, weight: t
     """x, residual: [..., N] bf16 or fp16 (residual None: the plain norm of x); weight [N] of
     the same type or fp32.  Returns (norm, x + residual), both contiguous in x's type;
     the second is x itself without a residual."""
-    M, N = _check(x, residual, weight, "fused_add_rms_norm")
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    h = x if residual is None else torch.empty_like(y)
-    if M == 0:
-        return y, h
-    w = _weight(weight)
-    xr, ldx = _row_pitch(x, M, N)
-    rr, ldr = (None, 0) if residual is None else _row_pitch(residual, M, N)
-    L.launch("qik_add_rms_norm", x.device, xr.data_ptr(), ldx, None if rr is None else rr.data_ptr(), ldr, w.data_ptr(),
-             w.dtype == torch.float32, M, N, eps, x.dtype == torch.float16,
-             None if residual is None else h.data_ptr(), y.data_ptr())
+    xr, ldx, r, ldr, w, f32, M, N, keep = _prepare(x, residual, weight, "fused_add_rms_norm")
+    y = torch.empty_like(x, memory_format=torch.contiguous_format)
+    h = x if r is None else torch.empty_like(y)
+    if M:
+        L.launch("qik_add_rms_norm", x.device.index, xr.data_ptr(), ldx, r, ldr, w.data_ptr(), f32, M, N, eps,
+                 x.dtype == torch.float16, None if r is None else h.data_ptr(), y.data_ptr())
     return y, h
 
 
@@ -82,24 +82,27 @@ def fused_add_rms_norm_e4m3(x: torch.Tensor, residual: torch.Tensor | None, weig
     """As ``fused_add_rms_norm`` with the norm quantized: returns (codes e4m3 [..., N],
     scale fp32, x + residual).  ``scales="tensor"``: one scale, shape [1], which
     ``FP8Linear.forward_e4m3`` takes; ``scales="row"``: one for each row, shape [...]."""
-    M, N = _check(x, residual, weight, "fused_add_rms_norm_e4m3")
-    if scales not in ("tensor", "row"):
-        raise ValueError(f"qik: fused_add_rms_norm_e4m3: scales is 'tensor' or 'row', got {scales!r}")
-    by_row = scales == "row"
-    dev = x.device
-    q = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=dev)
-    h = x if residual is None else torch.empty(x.shape, dtype=x.dtype, device=dev)
-    s = torch.empty(x.shape[:-1] if by_row else 1, dtype=torch.float32, device=dev)
-    if M == 0:
-        if not by_row:
+    xr, ldx, r, ldr, w, f32, M, N, keep = _prepare(x, residual, weight, "fused_add_rms_norm_e4m3")
+    idx = x.device.index
+    q = torch.empty_like(x, dtype=torch.float8_e4m3fn, memory_format=torch.contiguous_format)
+    h = x if r is None else torch.empty_like(x, memory_format=torch.contiguous_format)
+    ws, by_row = None, scales == "row"
+    if by_row:
+        s = x.new_empty(x.shape[:-1], dtype=torch.float32)
+    elif scales == "tensor":
+        one = _one.get(idx)
+        if one is None:
+            one = _one[idx] = torch.empty(1, dtype=torch.float32, device=x.device)
+        s = torch.empty_like(one)
+        if M == 0:
             s.fill_(1e-12)
-        return q, s, h
-    w = _weight(weight)
-    xr, ldx = _row_pitch(x, M, N)
-    rr, ldr = (None, 0) if residual is None else _row_pitch(residual, M, N)
-    ws = None if by_row else torch.empty(L.load().qik_add_rms_norm_workspace_bytes(M), dtype=torch.uint8, device=dev)
-    L.launch("qik_add_rms_norm_e4m3", dev, xr.data_ptr(), ldx, None if rr is None else rr.data_ptr(), ldr, w.data_ptr(),
-             w.dtype == torch.float32, M, N, eps, x.dtype == torch.float16,
-             None if residual is None else h.data_ptr(), q.data_ptr(), s.data_ptr(), by_row,
-             None if ws is None else ws.data_ptr())
+        else:
+            n = L.on_device("qik_add_rms_norm_workspace_bytes", idx, M, N)
+            ws = x.new_empty(n, dtype=torch.uint8) if n else None
+    else:
+        raise ValueError(f"qik: fused_add_rms_norm_e4m3: scales is 'tensor' or 'row', got {scales!r}")
+    if M:
+        L.launch("qik_add_rms_norm_e4m3", idx, xr.data_ptr(), ldx, r, ldr, w.data_ptr(), f32, M, N, eps,
+                 x.dtype == torch.float16, None if r is None else h.data_ptr(), q.data_ptr(), s.data_ptr(), by_row,
+                 None if ws is None else ws.data_ptr())
     return q, s, h

@@ -10,7 +10,6 @@ the turned k and v in the pages of a cache (``qik.paged_kv``) in the same kernel
 """
 from __future__ import annotations
 
-import ctypes
 import math
 
 import torch
@@ -76,50 +75,70 @@ def rotary_table(rotary_dim: int, max_positions: int, *, device: torch.device | 
     return (angle.cos() * gain).float(), (angle.sin() * gain).float()
 
 
-def _heads(t: torch.Tensor, name: str, like: torch.Tensor) -> torch.Tensor:
-    """t as [T, H, D] with a unit column stride, 16-byte rows and heads (copied otherwise)."""
-    if t.dim() != 3 or t.dtype != like.dtype or t.device != like.device or t.shape[0] != like.shape[0] or \
-            t.shape[2] != like.shape[2]:
-        raise ValueError(f"qik: {name} is {tuple(t.shape)} {t.dtype} on {t.device}: expected [{like.shape[0]}, heads, "
-                         f"{like.shape[2]}] {like.dtype} on {like.device}")
+def _heads(t: torch.Tensor, name: str, T: int, D: int, dtype: torch.dtype, dev: torch.device) -> tuple:
+    """t as [T, H, D] with a unit column stride, 16-byte rows and heads (copied otherwise), and
+    its heads, token and head strides."""
+    s = t.shape
+    if len(s) != 3 or s[0] != T or s[2] != D or t.dtype != dtype or t.device != dev:
+        raise ValueError(f"qik: {name} is {tuple(s)} {t.dtype} on {t.device}: expected [{T}, heads, {D}] {dtype} on {dev}")
     st, sh, sd = t.stride()
-    if sd != 1 or st % 8 or sh % 8 or t.data_ptr() % 16:
-        return t.clone(memory_format=torch.contiguous_format)
-    return t
+    if sd != 1 or (st | sh) % 8 or t.data_ptr() % 16:
+        t = t.clone(memory_format=torch.contiguous_format)
+        st, sh, sd = t.stride()
+    return t, s[1], st, sh
 
 
-def _index(t: torch.Tensor, name: str, like: torch.Tensor) -> torch.Tensor:
-    if t.dtype not in _INTS or t.device != like.device or t.dim() != 1 or t.shape[0] != like.shape[0]:
-        raise ValueError(f"qik: {name} is {tuple(t.shape)} {t.dtype} on {t.device}: expected [{like.shape[0]}] int32 or "
-                         f"int64 on {like.device}")
+def _index(t: torch.Tensor, name: str, T: int, dev: torch.device) -> torch.Tensor:
+    if t.shape != (T,) or t.dtype not in _INTS or t.device != dev:
+        raise ValueError(f"qik: {name} is {tuple(t.shape)} {t.dtype} on {t.device}: expected [{T}] int32 or int64 on {dev}")
     return t if t.is_contiguous() else t.contiguous()
 
 
-def _args(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, table: tuple, interleaved: bool) -> tuple:
+def _run(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor | None, positions: torch.Tensor, table: tuple,
+         slots: torch.Tensor | None, k_out: torch.Tensor | None, v_out: torch.Tensor | None, interleaved: bool) -> tuple:
     if not q.is_cuda:
         raise ValueError("qik: q must be a CUDA tensor (the kernels have no CPU path)")
-    if q.dtype not in _FLOATS:
-        raise TypeError(f"qik: rotary: bf16 or fp16, got {q.dtype}")
+    dtype, dev = q.dtype, q.device
+    if dtype not in _FLOATS:
+        raise TypeError(f"qik: rotary: bf16 or fp16, got {dtype}")
     if q.dim() != 3 or q.shape[2] not in (64, 128, 256):
         raise ValueError(f"qik: q is {tuple(q.shape)}: expected [tokens, heads, 64, 128 or 256]")
+    T, HQ, D = q.shape
     cos, sin = table
-    if cos.dtype != torch.float32 or sin.dtype != torch.float32 or cos.shape != sin.shape or cos.dim() != 2 or \
-            not (cos.is_contiguous() and sin.is_contiguous()) or cos.device != q.device or sin.device != q.device:
+    P, pairs = cos.shape if cos.dim() == 2 else (0, 0)
+    if cos.dtype != torch.float32 or sin.dtype != torch.float32 or sin.shape != cos.shape or P == 0 or \
+            not (cos.is_contiguous() and sin.is_contiguous()) or cos.device != dev or sin.device != dev:
         raise ValueError("qik: table is (cos, sin), contiguous fp32 [positions, rotary_dim / 2] on q's device")
-    rot = 2 * cos.shape[1]
-    if rot % 16 or not 0 < rot <= q.shape[2] or cos.shape[0] == 0:
-        raise ValueError(f"qik: a table for {rot} columns does not fit heads of {q.shape[2]} (a multiple of 16)")
-    q, k, positions = _heads(q, "q", q), _heads(k, "k", q), _index(positions, "positions", q)
-    a = L.RotaryArgs()
-    a.q, a.k, a.positions, a.cos, a.sin = (q.data_ptr(), k.data_ptr(), positions.data_ptr(), cos.data_ptr(),
-                                           sin.data_ptr())
-    a.T, a.HQ, a.D = q.shape
-    a.HK, a.rot, a.P = k.shape[1], rot, cos.shape[0]
-    a.q_st, a.q_sh, _ = q.stride()
-    a.k_st, a.k_sh, _ = k.stride()
-    a.flags = ((L.ROTARY_INTERLEAVED if interleaved else 0) | (L.ROTARY_F16 if q.dtype == torch.float16 else 0)
-               | (L.ROTARY_POS64 if positions.dtype == torch.int64 else 0))
-    return a, q, k, positions
+    if pairs == 0 or pairs % 8 or 2 * pairs > D:
+        raise ValueError(f"qik: a table for {2 * pairs} columns does not fit heads of {D} (a multiple of 16)")
+    q, _, q_st, q_sh = _heads(q, "q", T, D, dtype, dev)
+    k, HK, k_st, k_sh = _heads(k, "k", T, D, dtype, dev)
+    positions = _index(positions, "positions", T, dev)
+    flags = ((L.ROTARY_INTERLEAVED if interleaved else 0) | (L.ROTARY_F16 if dtype == torch.float16 else 0)
+             | (L.ROTARY_POS64 if positions.dtype == torch.int64 else 0))
+    q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    if slots is None:
+        k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
+        v_ptr = v_out_ptr = slots_ptr = 0
+        v_st = v_sh = page = pages = 0
+        strides = (0, 0, 0, 0, 0, 0)
+    else:
+        v, HV, v_st, v_sh = _heads(v, "v", T, D, dtype, dev)
+        if HV != HK:
+            raise ValueError(f"qik: v has {HV} heads, k {HK}")
+        slots = _index(slots, "slots", T, dev)
+        pages, heads, page, strides = check_pages(k_out, v_out, D, dtype, dev)
+        if heads != HK:
+            raise ValueError(f"qik: pages hold {heads} heads, k has {HK}")
+        flags |= L.ROTARY_PAGED | (L.ROTARY_SLOT64 if slots.dtype == torch.int64 else 0)
+        v_ptr, v_out_ptr, slots_ptr = v.data_ptr(), v_out.data_ptr(), slots.data_ptr()
+    idx = dev.index
+    if T:
+        L.launch("qik_rotary", idx,
+                 L.pack_rotary(q.data_ptr(), k.data_ptr(), v_ptr, q_out.data_ptr(), k_out.data_ptr(), v_out_ptr,
+                               positions.data_ptr(), slots_ptr, cos.data_ptr(), sin.data_ptr(), T, HQ, HK, D, 2 * pairs, P,
+                               q_st, q_sh, k_st, k_sh, v_st, v_sh, page, pages, *strides, flags), L.status_ptr(idx))
+    return q_out, k_out
 
 
 def apply_rotary(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, table: tuple[torch.Tensor, torch.Tensor],
@@ -128,12 +147,7 @@ def apply_rotary(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, tabl
     a fused projection are read in place); positions [T] int32 or int64; table from
     ``rotary_table``.  Returns the turned q and k, contiguous.  A position outside the
     table gives zeros and ``STATUS_BAD_INDEX`` in the device's status word."""
-    a, q, k, positions = _args(q, k, positions, table, interleaved)
-    q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-    a.q_out, a.k_out = q_out.data_ptr(), k_out.data_ptr()
-    L.launch("qik_rotary", q.device, ctypes.byref(a), L.status_word(q.device).data_ptr())
-    return q_out, k_out
+    return _run(q, k, None, positions, table, None, None, None, interleaved)
 
 
 def rotary_store(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor,
@@ -143,37 +157,23 @@ def rotary_store(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: t
     page, D] (page a power of two): token t at page slots[t] // page, place slots[t] % page.
     slots [T] int32 or int64, distinct; a negative slot stores nothing (padding), one behind the
     last page stores nothing and sets ``STATUS_BAD_INDEX``.  Returns the turned q."""
-    a, q, k, positions = _args(q, k, positions, table, interleaved)
-    v, slots = _heads(v, "v", q), _index(slots, "slots", q)
-    if v.shape != k.shape:
-        raise ValueError(f"qik: v is {tuple(v.shape)}, k {tuple(k.shape)}")
-    check_pages(k_pages, v_pages, q, k.shape[1])
-    pages, _, page, _ = k_pages.shape
-    q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    a.q_out, a.k_out, a.v_out, a.v, a.slots = (q_out.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), v.data_ptr(),
-                                               slots.data_ptr())
-    a.v_st, a.v_sh, _ = v.stride()
-    a.page, a.pages = page, pages
-    a.kp_s0, a.kp_sh, a.kp_ss, _ = k_pages.stride()
-    a.vp_s0, a.vp_sh, a.vp_ss, _ = v_pages.stride()
-    a.flags |= L.ROTARY_PAGED | (L.ROTARY_SLOT64 if slots.dtype == torch.int64 else 0)
-    L.launch("qik_rotary", q.device, ctypes.byref(a), L.status_word(q.device).data_ptr())
-    return q_out
+    return _run(q, k, v, positions, table, slots, k_pages, v_pages, interleaved)[0]
 
 
-def check_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, like: torch.Tensor, heads: int | None = None) -> None:
-    """One layer's page pools: [pages, heads, page, D] of like's type and device, page a power of
-    two of at least 16 tokens, unit column stride and 16-byte strides."""
+def check_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, D: int, dtype: torch.dtype, dev: torch.device) -> tuple:
+    """One layer's page pools: [pages, heads, page, D], page a power of two of 16 to 4096 tokens,
+    unit column stride, 16-byte strides.  Returns pages, heads, page and the page, head and token
+    strides of both."""
     s = k_pages.shape
-    if v_pages.shape != s or len(s) != 4 or k_pages.dtype != like.dtype or v_pages.dtype != like.dtype or \
-            k_pages.device != like.device or v_pages.device != like.device or s[3] != like.shape[-1]:
-        raise ValueError(f"qik: pages {tuple(s)} {k_pages.dtype} and {tuple(v_pages.shape)} {v_pages.dtype}: expected two "
-                         f"[pages, heads, page, {like.shape[-1]}] {like.dtype} on {like.device}")
-    if heads is not None and s[1] != heads:
-        raise ValueError(f"qik: pages hold {s[1]} heads, k has {heads}")
-    if s[0] == 0 or s[1] == 0 or s[2] < 16 or s[2] > 4096 or s[2] & (s[2] - 1):
+    if len(s) != 4 or v_pages.shape != s or s[3] != D or k_pages.dtype != dtype or v_pages.dtype != dtype or \
+            k_pages.device != dev or v_pages.device != dev:
+        raise ValueError(f"qik: pages {tuple(s)} {k_pages.dtype} on {k_pages.device} and {tuple(v_pages.shape)} "
+                         f"{v_pages.dtype} on {v_pages.device}: expected two [pages, heads, page, {D}] {dtype} on {dev}")
+    pages, heads, page, _ = s
+    if pages == 0 or heads == 0 or page < 16 or page > 4096 or page & (page - 1):
         raise ValueError(f"qik: pages {tuple(s)}: a page is a power of two of 16 to 4096 tokens")
-    for t in (k_pages, v_pages):
-        a, b, c, d = t.stride()
-        if d != 1 or a % 8 or b % 8 or c % 8 or min(a, b, c) < 0 or t.data_ptr() % 16:
-            raise ValueError("qik: pages need a unit column stride, strides of 16 bytes and 16-byte alignment")
+    a, b, c, d = k_pages.stride()
+    e, f, g, h = v_pages.stride()
+    if d != 1 or h != 1 or (a | b | c | e | f | g) % 8 or (k_pages.data_ptr() | v_pages.data_ptr()) % 16:
+        raise ValueError("qik: pages need a unit column stride, strides of 16 bytes and 16-byte alignment")
+    return pages, heads, page, (a, b, c, e, f, g)

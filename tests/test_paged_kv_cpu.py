@@ -143,11 +143,11 @@ def _fails(lib, rc, text):
 def test_copy_pages_refuses_bad_moves(lib):
     """The list is checked before anything is launched."""
     from qik import _lib as L
-    p = L.PagePools(4096, 8192, 2, 10, 2, 16, 128, 10 * 4096, 4096, 2048, 10 * 4096, 4096, 2048)
+    p = L.pack_pools(4096, 8192, 2, 10, 2, 16, 128, 10 * 4096, 4096, 2048, 10 * 4096, 4096, 2048)
 
-    def call(*moves):
+    def call(*moves, p=p):
         flat = (ctypes.c_int32 * (3 * len(moves)))(*[x for m in moves for x in m])
-        return lib.qik_copy_pages(ctypes.byref(p), flat, len(moves), None)
+        return lib.qik_copy_pages(p, flat, len(moves), None)
     _fails(lib, call((0, 10, 1)), "outside 10 pages")
     _fails(lib, call((-1, 1, 1)), "outside 10 pages")
     _fails(lib, call((0, 1, 17)), "outside 10 pages")
@@ -156,16 +156,16 @@ def test_copy_pages_refuses_bad_moves(lib):
     _fails(lib, call((0, 1, 1), (1, 2, 1)), "both read and written")
     _fails(lib, call((3, 3, 1)), "both read and written")
     assert call((0, 1, 0)) == 0  # nothing to copy
-    assert lib.qik_copy_pages(ctypes.byref(p), None, 0, None) == 0
-    _fails(lib, lib.qik_copy_pages(ctypes.byref(p), None, 1, None), "NULL")
-    p.token_bytes = 100
-    _fails(lib, call((0, 1, 1)), "16 bytes")
+    assert lib.qik_copy_pages(p, None, 0, None) == 0
+    _fails(lib, lib.qik_copy_pages(p, None, 1, None), "NULL")
+    odd = L.pack_pools(4096, 8192, 2, 10, 2, 16, 100, 10 * 4096, 4096, 2048, 10 * 4096, 4096, 2048)
+    _fails(lib, call((0, 1, 1), p=odd), "16 bytes")
 
 
 def test_norm_entry_refusals(lib):
     x = ctypes.c_void_p(4096)
 
-    def call(M=4, N=64, ldx=64, ldr=64, eps=1e-6, y=x, scale=x, ws=x):
+    def call(M=20, N=64, ldx=64, ldr=64, eps=1e-6, y=x, scale=x, ws=x):
         return lib.qik_add_rms_norm_e4m3(x, ldx, x, ldr, x, 0, M, N, eps, 0, x, y, scale, 0, ws, None)
     _fails(lib, call(N=60), "60 columns")
     _fails(lib, call(N=32776, ldx=32776), "32776 columns")
@@ -177,21 +177,18 @@ def test_norm_entry_refusals(lib):
     _fails(lib, call(eps=-1.0), "eps")
     _fails(lib, call(y=ctypes.c_void_p(4104)), "aligned")
     assert call(M=0) == 0
-    assert lib.qik_add_rms_norm_workspace_bytes(100) >= 400
+    assert lib.qik_add_rms_norm_workspace_bytes(100, 64) >= 400 and lib.qik_add_rms_norm_workspace_bytes(3, 64) == 0
 
 
 def test_rotary_entry_refusals(lib):
     from qik import _lib as L
 
     def call(**kw):
-        a = L.RotaryArgs()
         base = dict(q=4096, k=4096, v=4096, q_out=4096, k_out=4096, v_out=4096, positions=4096, slots=4096, cos=4096, sin=4096,
                     T=4, HQ=4, HK=2, D=128, rot=128, P=100, q_st=512, q_sh=128, k_st=256, k_sh=128, v_st=256, v_sh=128,
                     page=16, pages=4, kp_s0=4096, kp_sh=2048, kp_ss=128, vp_s0=4096, vp_sh=2048, vp_ss=128,
                     flags=L.ROTARY_PAGED)
-        for k, v in (base | kw).items():
-            setattr(a, k, v)
-        return lib.qik_rotary(ctypes.byref(a), None, None)
+        return lib.qik_rotary(L.pack_rotary(*[0 if x is None else x for x in (base | kw).values()]), None, None)
     for kw, text in ((dict(D=96), "head_dim"), (dict(rot=136), "rotated"), (dict(rot=24), "rotated"), (dict(P=0), "positions"),
                      (dict(q=None), "NULL"), (dict(v=None), "paged"), (dict(slots=None), "paged"), (dict(q_st=4), "strides"),
                      (dict(page=24), "power of two"), (dict(kp_ss=4), "page strides"), (dict(k=4100), "aligned"),
@@ -204,14 +201,12 @@ def test_attention_entry_refusals(lib):
     from qik import _lib as L
 
     def call(ws=4096, ws_bytes=1 << 40, **kw):
-        a = L.PagedAttnArgs()
         base = dict(q=4096, k_pages=4096, v_pages=4096, out=4096, page_table=4096, seq_lens=4096, query_starts=4096, B=2, T=4,
                     HQ=4, HK=2, D=128, W=10, pages=30, page=16, max_new=2, max_kv=160, q_st=512, q_sh=128, o_st=512, o_sh=128,
                     table_st=10, kp_s0=4096, kp_sh=2048, kp_ss=128, vp_s0=4096, vp_sh=2048, vp_ss=128, sm_scale=0.1,
                     window=0, sinks=0, flags=L.PAGED_CAUSAL)
-        for k, v in (base | kw).items():
-            setattr(a, k, v)
-        return lib.qik_paged_attention(ctypes.byref(a), ws, ws_bytes, None, None)
+        a = L.pack_paged_attn(*[0 if x is None else x for x in (base | kw).values()])
+        return lib.qik_paged_attention(a, ws, ws_bytes, None, None)
     for kw, text in ((dict(D=96), "head_dim"), (dict(HQ=5), "bad sizes"), (dict(page=24), "power of two"), (dict(page=8), "power of two"),
                      (dict(W=1 << 27), "page table"), (dict(max_new=5), "max_new"), (dict(max_kv=-1), "max_kv"),
                      (dict(window=-1), "window"), (dict(window=4, flags=0), "causal"), (dict(sm_scale=0.0), "sm_scale"),
@@ -261,3 +256,24 @@ def test_rotary_scalings():
         rotary_frequencies(63)
     with pytest.raises(ValueError):
         rotary_table(64, 0, device="cpu")
+
+
+def test_packed_structs_match_the_header(tmp_path):
+    """The packers of qik/_lib.py lay their fields out as a C compiler lays out include/qik.h."""
+    import subprocess
+
+    from conftest import ROOT
+    from qik import _lib as L
+    c = tmp_path / "sizes.c"
+    c.write_text('#include <stddef.h>\n#include <stdio.h>\n#include "qik.h"\nint main(void) {\n'
+                 'printf("%zu %zu %zu %zu %zu %zu\\n", sizeof(qik_rotary_args), offsetof(qik_rotary_args, kp_s0), '
+                 'sizeof(qik_page_pools), sizeof(qik_paged_attn_args), offsetof(qik_paged_attn_args, sm_scale), '
+                 'offsetof(qik_paged_attn_args, max_kv));\nreturn 0;\n}\n')
+    subprocess.run(["gcc", "-I", str(ROOT / "include"), str(c), "-o", str(tmp_path / "sizes")], check=True)
+    said = [int(x) for x in subprocess.run([str(tmp_path / "sizes")], check=True, capture_output=True, text=True).stdout.split()]
+    rotary = L.pack_rotary(*range(1, 32))
+    attn = L.pack_paged_attn(*range(1, 29), 0.5, *range(30, 33))
+    assert said[0] == len(rotary) and int.from_bytes(rotary[said[1]:said[1] + 8], "little") == 25
+    assert said[2] == len(L.pack_pools(*range(13))) and said[3] == len(attn)
+    import struct
+    assert struct.unpack_from("f", attn, said[4])[0] == 0.5 and int.from_bytes(attn[said[5]:said[5] + 8], "little") == 17
