@@ -6,6 +6,9 @@ Each .cu under csrc/ is compiled by nvcc to an object (in csrc/_build/) and link
 into qik/libqik.so with the CUDA runtime linked statically, so the library has no
 dependency beyond the driver.  Objects are rebuilt when their source or any header
 is newer.
+
+The host calls of the decoder operators (csrc/calls.cpp) are a CPython module over torch's
+C++ tensors, compiled by g++ to qik/_calls.so and linked against libqik.so beside it.
 """
 from __future__ import annotations
 
@@ -21,6 +24,7 @@ CSRC = HERE / "csrc"
 OBJ = CSRC / "_build"
 INCLUDE = HERE.parent / "include"
 OUT = HERE / "qik" / "libqik.so"
+CALLS = HERE / "qik" / "_calls.so"
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr", "-Xptxas",
@@ -56,7 +60,27 @@ def build(force: bool = False, verbose_ptxas: bool = False) -> Path:
         cmd = [nvcc(), *ARCH, "-shared", "-cudart", "static", "-o", str(OUT), *map(str, objs)]
         print("[qik build] link", OUT.name, flush=True)
         subprocess.run(cmd, check=True)
+    build_calls(force)
     return OUT
+
+
+def build_calls(force: bool = False) -> Path:
+    import sysconfig
+
+    import torch
+    src, header = CSRC / "calls.cpp", INCLUDE / "qik.h"
+    if not force and CALLS.exists() and CALLS.stat().st_mtime >= max(src.stat().st_mtime, header.stat().st_mtime):
+        return CALLS
+    root = Path(torch.__file__).resolve().parent
+    cuda = Path(nvcc()).resolve().parent.parent
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           "-I", str(INCLUDE), "-isystem", str(root / "include"), "-isystem", str(root / "include/torch/csrc/api/include"),
+           "-isystem", sysconfig.get_paths()["include"], "-isystem", str(cuda / "include"), str(src), "-o", str(CALLS),
+           "-L", str(root / "lib"), "-ltorch_python", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda",
+           "-L", str(OUT.parent), "-l:libqik.so", "-Wl,-rpath,$ORIGIN"]
+    print("[qik build] g++", src.name, flush=True)
+    subprocess.run(cmd, check=True)
+    return CALLS
 
 
 if __name__ == "__main__":

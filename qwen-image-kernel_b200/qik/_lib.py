@@ -7,7 +7,6 @@ raises instead of computing anything elsewhere.
 from __future__ import annotations
 
 import ctypes
-import struct
 import threading
 from pathlib import Path
 
@@ -21,8 +20,6 @@ EPI_SCALE, EPI_GELU_TANH, EPI_SCATTER, EPI_SWIGLU = 0, 1, 2, 3
 GEMM_TILE_AUTO, GEMM_TILE_PAIR_256, GEMM_TILE_SINGLE_256, GEMM_TILE_SINGLE_128, GEMM_TILE_SINGLE_64, GEMM_TILE_SWAP_16 = range(6)
 TP_MAX_WORLD = 8
 ATTN_HAS_CACHE, ATTN_HAS_KEY_VALID, ATTN_UNIFORM, ATTN_V_FP8, ATTN_F16 = 1, 2, 4, 8, 16
-ROTARY_INTERLEAVED, ROTARY_F16, ROTARY_PAGED, ROTARY_POS64, ROTARY_SLOT64 = 1, 2, 4, 8, 16
-PAGED_CAUSAL, PAGED_F16 = 1, 2
 STATUS_OK, STATUS_TIMEOUT, STATUS_BAD_INDEX = 0, 1, 2
 
 _i64, _i32, _f32, _vp, _u64 = ctypes.c_int64, ctypes.c_int, ctypes.c_float, ctypes.c_void_p, ctypes.c_uint64
@@ -45,20 +42,6 @@ class AttnArgs(ctypes.Structure):
         ("flags", _i32),
         ("amax_out", _vp),
     ]
-
-
-# The structs of the calls that a decoder makes in every layer, as packers: one call packs
-# the fields in the order of include/qik.h (native alignment), several times faster than a
-# ctypes.Structure; the bytes are passed where the entry point takes a pointer.
-# qik_rotary_args: q k v q_out k_out v_out positions slots cos sin | T HQ HK D rot P |
-#   q_st q_sh k_st k_sh v_st v_sh | page pages | kp_s0 kp_sh kp_ss vp_s0 vp_sh vp_ss | flags
-pack_rotary = struct.Struct("@10P20qi0q").pack
-# qik_page_pools: k v | layers pages heads page token_bytes | k layer, page, head bytes | v ...
-pack_pools = struct.Struct("@2P11q").pack
-# qik_paged_attn_args: q k_pages v_pages out page_table seq_lens query_starts | B T HQ HK D W
-#   pages page max_new max_kv | q_st q_sh o_st o_sh table_st | kp_s0 kp_sh kp_ss vp_s0 vp_sh vp_ss |
-#   sm_scale | window sinks flags
-pack_paged_attn = struct.Struct("@7P21qf3i0q").pack
 
 
 # name -> (restype, argtypes)
@@ -167,35 +150,11 @@ def stream_ptr(device: torch.device | None = None) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
-def on_device(name: str, idx: int, *args):
-    """What the entry point ``name`` returns for ``args`` with device ``idx`` current (its answer
-    may depend on that device's SMs)."""
-    fn = getattr(_lib or load(), name)
-    if torch._C._cuda_getDevice() == idx:
-        return fn(*args)
-    with torch.cuda.device(idx):
-        return fn(*args)
-
-
-def launch(name: str, idx: int, *args) -> None:
-    """Call the entry point ``name`` with ``args`` and the current stream of device ``idx``, with
-    that device current (its tensors need not be on the current one)."""
-    fn = getattr(_lib or load(), name)
-    if torch._C._cuda_getDevice() == idx:
-        rc = fn(*args, torch._C._cuda_getCurrentRawStream(idx))
-    else:
-        with torch.cuda.device(idx):
-            rc = fn(*args, torch._C._cuda_getCurrentRawStream(idx))
-    if rc != QIK_OK:
-        check(rc, name)
-
-
 def ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 
 
 _status: dict[int, torch.Tensor] = {}
-_status_ptr: dict[int, int] = {}
 
 
 def status_word(device: torch.device) -> torch.Tensor:
@@ -209,11 +168,8 @@ def status_word(device: torch.device) -> torch.Tensor:
 
 
 def status_ptr(idx: int) -> int:
-    """Address of device ``idx``'s status word."""
-    p = _status_ptr.get(idx)
-    if p is None:
-        p = _status_ptr[idx] = status_word(torch.device("cuda", idx)).data_ptr()
-    return p
+    """Address of device ``idx``'s status word (for qik._calls, which keeps it)."""
+    return status_word(torch.device("cuda", idx)).data_ptr()
 
 
 def device_status(device: torch.device | None = None) -> int:

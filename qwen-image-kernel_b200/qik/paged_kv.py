@@ -16,7 +16,7 @@ import heapq
 import numpy as np
 import torch
 
-from . import _lib as L
+from . import _calls
 
 
 class CacheFull(RuntimeError):
@@ -27,40 +27,12 @@ def copy_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, moves) -> None:
     """Copy the first tokens of pages to other pages, in every layer and head of both pools.
 
     k_pages, v_pages: [layers, pages, heads, page, D] (or one layer's [pages, heads, page, D]);
-    moves: a sequence of (from, to, tokens), or an int array [n, 3], on the host.  The rest of a
+    moves: a list of (from, to, tokens), or an int array or tensor [n, 3].  The rest of a
     written page stays as it is.  No page may be written twice or both read and written in one
     call; indices are checked before anything is launched."""
-    if not k_pages.is_cuda:
-        raise ValueError("qik: k_pages must be a CUDA tensor (the kernels have no CPU path)")
-    if k_pages.shape != v_pages.shape or k_pages.dtype != v_pages.dtype or k_pages.device != v_pages.device or \
-            k_pages.dim() not in (4, 5):
-        raise ValueError(f"qik: pages {tuple(k_pages.shape)} {k_pages.dtype} and {tuple(v_pages.shape)} {v_pages.dtype}: "
-                         "expected two [layers, pages, heads, page, D] of one type on one device")
-    if isinstance(moves, torch.Tensor):
-        if moves.is_cuda:
-            raise ValueError("qik: copy_pages takes its moves on the host")
-        moves = moves.numpy()
-    wide = np.asarray(moves)
-    if wide.size == 0:
-        return
-    if wide.ndim != 2 or wide.shape[1] != 3 or wide.dtype.kind not in "iu":
-        raise ValueError("qik: moves is a sequence of (from, to, tokens)")
-    if wide.dtype == np.int32 and wide.flags.c_contiguous:
-        m = wide
-    else:
-        if wide.max() > 0x7FFFFFFF or wide.min() < 0:
-            raise ValueError("qik: copy_pages: a move is outside the pool")
-        m = wide.astype(np.int32, order="C")
-    size = k_pages.element_size()
-    shape, ks, vs = k_pages.shape, k_pages.stride(), v_pages.stride()
-    if len(shape) == 4:
-        shape, ks, vs = (1, *shape), (0, *ks), (0, *vs)
-    layers, pages, heads, page, D = shape
-    if ks[4] != 1 or vs[4] != 1 or ks[3] != D or vs[3] != D:
-        raise ValueError("qik: a head's tokens must be contiguous in a page")
-    L.launch("qik_copy_pages", k_pages.device.index,
-             L.pack_pools(k_pages.data_ptr(), v_pages.data_ptr(), layers, pages, heads, page, D * size, ks[0] * size,
-                          ks[1] * size, ks[2] * size, vs[0] * size, vs[1] * size, vs[2] * size), m.ctypes.data, len(m))
+    if not isinstance(moves, (list, tuple)):
+        moves = moves.tolist()
+    _calls.copy_pages(k_pages, v_pages, moves)
 
 
 class PagedStep:

@@ -2,9 +2,23 @@
 import ctypes
 import math
 import random
+import struct
 
 import pytest
 import torch
+
+# The argument structs of include/qik.h, in its order (native alignment):
+# qik_rotary_args: q k v q_out k_out v_out positions slots cos sin | T HQ HK D rot P |
+#   q_st q_sh k_st k_sh v_st v_sh | page pages | kp_s0 kp_sh kp_ss vp_s0 vp_sh vp_ss | flags
+pack_rotary = struct.Struct("@10P20qi0q").pack
+# qik_page_pools: k v | layers pages heads page token_bytes | k layer, page, head bytes | v ...
+pack_pools = struct.Struct("@2P11q").pack
+# qik_paged_attn_args: q k_pages v_pages out page_table seq_lens query_starts | B T HQ HK D W
+#   pages page max_new max_kv | q_st q_sh o_st o_sh table_st | kp_s0 kp_sh kp_ss vp_s0 vp_sh vp_ss |
+#   sm_scale | window sinks flags
+pack_paged_attn = struct.Struct("@7P21qf3i0q").pack
+PAGED = 4    # QIK_ROTARY_PAGED
+CAUSAL = 1   # QIK_PAGED_CAUSAL
 
 
 @pytest.fixture
@@ -142,8 +156,7 @@ def _fails(lib, rc, text):
 
 def test_copy_pages_refuses_bad_moves(lib):
     """The list is checked before anything is launched."""
-    from qik import _lib as L
-    p = L.pack_pools(4096, 8192, 2, 10, 2, 16, 128, 10 * 4096, 4096, 2048, 10 * 4096, 4096, 2048)
+    p = pack_pools(4096, 8192, 2, 10, 2, 16, 128, 10 * 4096, 4096, 2048, 10 * 4096, 4096, 2048)
 
     def call(*moves, p=p):
         flat = (ctypes.c_int32 * (3 * len(moves)))(*[x for m in moves for x in m])
@@ -158,7 +171,7 @@ def test_copy_pages_refuses_bad_moves(lib):
     assert call((0, 1, 0)) == 0  # nothing to copy
     assert lib.qik_copy_pages(p, None, 0, None) == 0
     _fails(lib, lib.qik_copy_pages(p, None, 1, None), "NULL")
-    odd = L.pack_pools(4096, 8192, 2, 10, 2, 16, 100, 10 * 4096, 4096, 2048, 10 * 4096, 4096, 2048)
+    odd = pack_pools(4096, 8192, 2, 10, 2, 16, 100, 10 * 4096, 4096, 2048, 10 * 4096, 4096, 2048)
     _fails(lib, call((0, 1, 1), p=odd), "16 bytes")
 
 
@@ -181,14 +194,12 @@ def test_norm_entry_refusals(lib):
 
 
 def test_rotary_entry_refusals(lib):
-    from qik import _lib as L
-
     def call(**kw):
         base = dict(q=4096, k=4096, v=4096, q_out=4096, k_out=4096, v_out=4096, positions=4096, slots=4096, cos=4096, sin=4096,
                     T=4, HQ=4, HK=2, D=128, rot=128, P=100, q_st=512, q_sh=128, k_st=256, k_sh=128, v_st=256, v_sh=128,
                     page=16, pages=4, kp_s0=4096, kp_sh=2048, kp_ss=128, vp_s0=4096, vp_sh=2048, vp_ss=128,
-                    flags=L.ROTARY_PAGED)
-        return lib.qik_rotary(L.pack_rotary(*[0 if x is None else x for x in (base | kw).values()]), None, None)
+                    flags=PAGED)
+        return lib.qik_rotary(pack_rotary(*[0 if x is None else x for x in (base | kw).values()]), None, None)
     for kw, text in ((dict(D=96), "head_dim"), (dict(rot=136), "rotated"), (dict(rot=24), "rotated"), (dict(P=0), "positions"),
                      (dict(q=None), "NULL"), (dict(v=None), "paged"), (dict(slots=None), "paged"), (dict(q_st=4), "strides"),
                      (dict(page=24), "power of two"), (dict(kp_ss=4), "page strides"), (dict(k=4100), "aligned"),
@@ -198,14 +209,12 @@ def test_rotary_entry_refusals(lib):
 
 
 def test_attention_entry_refusals(lib):
-    from qik import _lib as L
-
     def call(ws=4096, ws_bytes=1 << 40, **kw):
         base = dict(q=4096, k_pages=4096, v_pages=4096, out=4096, page_table=4096, seq_lens=4096, query_starts=4096, B=2, T=4,
                     HQ=4, HK=2, D=128, W=10, pages=30, page=16, max_new=2, max_kv=160, q_st=512, q_sh=128, o_st=512, o_sh=128,
                     table_st=10, kp_s0=4096, kp_sh=2048, kp_ss=128, vp_s0=4096, vp_sh=2048, vp_ss=128, sm_scale=0.1,
-                    window=0, sinks=0, flags=L.PAGED_CAUSAL)
-        a = L.pack_paged_attn(*[0 if x is None else x for x in (base | kw).values()])
+                    window=0, sinks=0, flags=CAUSAL)
+        a = pack_paged_attn(*[0 if x is None else x for x in (base | kw).values()])
         return lib.qik_paged_attention(a, ws, ws_bytes, None, None)
     for kw, text in ((dict(D=96), "head_dim"), (dict(HQ=5), "bad sizes"), (dict(page=24), "power of two"), (dict(page=8), "power of two"),
                      (dict(W=1 << 27), "page table"), (dict(max_new=5), "max_new"), (dict(max_kv=-1), "max_kv"),
@@ -259,11 +268,10 @@ def test_rotary_scalings():
 
 
 def test_packed_structs_match_the_header(tmp_path):
-    """The packers of qik/_lib.py lay their fields out as a C compiler lays out include/qik.h."""
+    """The packers above lay their fields out as a C compiler lays out include/qik.h."""
     import subprocess
 
     from conftest import ROOT
-    from qik import _lib as L
     c = tmp_path / "sizes.c"
     c.write_text('#include <stddef.h>\n#include <stdio.h>\n#include "qik.h"\nint main(void) {\n'
                  'printf("%zu %zu %zu %zu %zu %zu\\n", sizeof(qik_rotary_args), offsetof(qik_rotary_args, kp_s0), '
@@ -271,9 +279,8 @@ def test_packed_structs_match_the_header(tmp_path):
                  'offsetof(qik_paged_attn_args, max_kv));\nreturn 0;\n}\n')
     subprocess.run(["gcc", "-I", str(ROOT / "include"), str(c), "-o", str(tmp_path / "sizes")], check=True)
     said = [int(x) for x in subprocess.run([str(tmp_path / "sizes")], check=True, capture_output=True, text=True).stdout.split()]
-    rotary = L.pack_rotary(*range(1, 32))
-    attn = L.pack_paged_attn(*range(1, 29), 0.5, *range(30, 33))
+    rotary = pack_rotary(*range(1, 32))
+    attn = pack_paged_attn(*range(1, 29), 0.5, *range(30, 33))
     assert said[0] == len(rotary) and int.from_bytes(rotary[said[1]:said[1] + 8], "little") == 25
-    assert said[2] == len(L.pack_pools(*range(13))) and said[3] == len(attn)
-    import struct
+    assert said[2] == len(pack_pools(*range(13))) and said[3] == len(attn)
     assert struct.unpack_from("f", attn, said[4])[0] == 0.5 and int.from_bytes(attn[said[5]:said[5] + 8], "little") == 17
