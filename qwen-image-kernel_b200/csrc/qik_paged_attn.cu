@@ -33,6 +33,7 @@
 // zeroed in shared memory before the product: whatever an unused place of a page holds,
 // NaN too, meets p = 0 there and would spread otherwise.
 #include <mutex>
+#include <type_traits>
 
 #include "qik_device.cuh"
 #include "qik_host.h"
@@ -312,21 +313,28 @@ __global__ void __launch_bounds__(SplitShape<D, MT>::kThreads, SplitShape<D, MT>
     while (more && ok) {
       const int count = static_cast<int>(min(static_cast<long long>(w.nt - w.at), w.left));
       const int32_t* row = a.table + static_cast<int64_t>(w.i) * a.table_st;
-      // a lane's page of tile u: behind the last token (or outside the table) none, which
-      // reads as zeros like any page outside the pool
-      auto page_of = [&](int u) {
-        if (lane >= pieces || u >= w.at + count || w.t.main == 0) return -1;
-        const int key = tile_at(w.t, u) * kSplitTile + lane * box;
+      // lane's page number for its piece of the tiles [u, u + 32 / pieces): one load serves them
+      // all, and the next is in flight while they are issued.  Behind the last token (or
+      // outside the table) there is none, which reads as zeros like any page outside the pool
+      auto page_of = [&](int u0) {
+        const int u = u0 + lane / pieces;
+        if (u >= w.at + count || w.t.main == 0) return -1;
+        const int key = tile_at(w.t, u) * kSplitTile + (lane % pieces) * box;
         const int p = key >> a.page_log2;
         if (key >= w.s.kv || p >= a.W) return -1;
         const int id = __ldg(row + p);
         if ((id < 0 || id >= a.pages) && a.status) atomicExch(a.status, QIK_DEV_BAD_INDEX);
         return id < a.pages ? id : -1;
       };
-      int next = page_of(w.at);
+      const int run = 32 / pieces;  // tiles that one load serves
+      int cur = 0, next = page_of(w.at);
       for (int u = w.at; u < w.at + count; ++u) {
-        const int id = next;
-        next = page_of(u + 1);
+        const int k = (u - w.at) % run;
+        if (k == 0) {
+          cur = next;
+          next = page_of(u + run);
+        }
+        const int id = __shfl_sync(0xffffffffu, cur, k * pieces + lane % pieces);
         if (!__all_sync(0xffffffffu, mbar_wait(&empty[stage], phase, abort_flag, a.status))) {
           ok = false;
           break;
@@ -549,58 +557,68 @@ __global__ void __launch_bounds__(SplitShape<D, MT>::kThreads, SplitShape<D, MT>
         named_bar_sync(1, Sh::kWarps * 32);
       }
       if (begins && !ends && threadIdx.x == 0)
-        a.ws_desc[blockIdx.x] = make_int4(w.i, w.h, static_cast<int>((w.nt - count + share - 1) / share), 0);
+        a.ws_desc[blockIdx.x] = make_int4(w.s.q0, w.h, static_cast<int>((w.nt - count + share - 1) / share), rows);
       more = walk_next(a, w, count);
     }
   }
   pdl_trigger();
 }
 
-// Joins the pieces of the unit that CTA blockIdx.x of the split kernel left open: its own
-// piece, then the following CTAs' first pieces, in that order.  One warp a row.
-template <int D, bool F16>
-__global__ void __launch_bounds__(512) paged_split_join_kernel(const PagedDev a, int slot_rows) {
-  pdl_wait();
-  const int4 d = __ldcg(a.ws_desc + blockIdx.x);
-  if (d.x < 0) return;
-  const Seq s = seq_of(a, d.x);
-  const int rows = s.n * a.G, lane = threadIdx.x & 31;
-  const int pieces = 1 + d.z;
-  auto row_of = [&](int p, int r) {
-    return static_cast<int64_t>(p == 0 ? 2 * blockIdx.x + 1 : 2 * (blockIdx.x + p)) * slot_rows + r;
-  };
-  for (int r = threadIdx.x >> 5; r < rows; r += 16) {
-    float top = -INFINITY, sum = 0.0f;
-    for (int p = lane; p < pieces; p += 32) top = fmaxf(top, __ldcg(a.ws_ml + row_of(p, r)).x);
+// sum_p f_p o_p / sum_p f_p l_p, f_p = 2^(m_p - max m), over the pieces of one row: `at(p)` is
+// piece p's row in the workspace.  One warp; lane holds D / 32 columns.  Pieces are added in
+// order, four loads in flight.
+template <int D, bool F16, typename At>
+__device__ __forceinline__ void join_row(const PagedDev& a, int pieces, At at, uint16_t* dst) {
+  using Vec = typename std::conditional<D == 128, float4, float2>::type;
+  const int lane = threadIdx.x & 31;
+  float top = -INFINITY, sum = 0.0f;
+  for (int p = lane; p < pieces; p += 32) top = fmaxf(top, __ldcg(a.ws_ml + at(p)).x);
+  float acc[D / 32];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    float acc[D / 32];
+  for (int c = 0; c < D / 32; ++c) acc[c] = 0.0f;
+  for (int p0 = 0; p0 < pieces; p0 += 4) {
+    float2 ml[4];
+    Vec v[4];
 #pragma unroll
-    for (int c = 0; c < D / 32; ++c) acc[c] = 0.0f;
-#pragma unroll 4
-    for (int p = 0; p < pieces; ++p) {
-      const int64_t at = row_of(p, r);
-      const float2 ml = __ldcg(a.ws_ml + at);
-      const float f = ml.x == -INFINITY ? 0.0f : ex2(ml.x - top);
-      sum = fmaf(ml.y, f, sum);
-      if (D == 128) {
-        const float4 v = __ldcg(reinterpret_cast<const float4*>(a.ws_o + at * D) + lane);
-        acc[0] = fmaf(v.x, f, acc[0]), acc[1] = fmaf(v.y, f, acc[1]);
-        acc[2] = fmaf(v.z, f, acc[2]), acc[3] = fmaf(v.w, f, acc[3]);
-      } else {
-        const float2 v = __ldcg(reinterpret_cast<const float2*>(a.ws_o + at * D) + lane);
-        acc[0] = fmaf(v.x, f, acc[0]), acc[1] = fmaf(v.y, f, acc[1]);
+    for (int k = 0; k < 4; ++k) {
+      const int64_t row = at(min(p0 + k, pieces - 1));
+      ml[k] = __ldcg(a.ws_ml + row);
+      v[k] = __ldcg(reinterpret_cast<const Vec*>(a.ws_o + row * D) + lane);
+    }
+    if (p0 == 0) {
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float f = p0 + k >= pieces || ml[k].x == -INFINITY ? 0.0f : ex2(ml[k].x - top);
+      if (p0 + k < pieces) {
+        sum = fmaf(ml[k].y, f, sum);
+        const float* e = reinterpret_cast<const float*>(&v[k]);
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) acc[c] = fmaf(e[c], f, acc[c]);
       }
     }
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    const int j = r / a.G, hq = d.y * a.G + r % a.G;
-    uint16_t* dst = a.out + static_cast<int64_t>(s.q0 + j) * a.o_st + static_cast<int64_t>(hq) * a.o_sh;
-    if (D == 128)
-      reinterpret_cast<uint2*>(dst)[lane] =
-          make_uint2(pack16<F16>(acc[0] * inv, acc[1] * inv), pack16<F16>(acc[2] * inv, acc[3] * inv));
-    else
-      reinterpret_cast<uint32_t*>(dst)[lane] = pack16<F16>(acc[0] * inv, acc[1] * inv);
   }
+  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+  if constexpr (D == 128)
+    reinterpret_cast<uint2*>(dst)[lane] =
+        make_uint2(pack16<F16>(acc[0] * inv, acc[1] * inv), pack16<F16>(acc[2] * inv, acc[3] * inv));
+  else
+    reinterpret_cast<uint32_t*>(dst)[lane] = pack16<F16>(acc[0] * inv, acc[1] * inv);
+}
+
+// Joins the pieces of the unit that CTA blockIdx.x of the split kernel left open: its own
+// piece, then the following CTAs' first pieces.  Four rows a CTA.
+template <int D, bool F16>
+__global__ void __launch_bounds__(128) paged_split_join_kernel(const PagedDev a, int slot_rows) {
+  pdl_wait();
+  const int4 d = __ldcg(a.ws_desc + blockIdx.x);  // first new token, head, further pieces, rows
+  const int r = blockIdx.y * 4 + (threadIdx.x >> 5);
+  if (d.x >= 0 && r < d.w)
+    join_row<D, F16>(a, 1 + d.z, [&](int p) {
+      return static_cast<int64_t>(p == 0 ? 2 * blockIdx.x + 1 : 2 * (blockIdx.x + p)) * slot_rows + r;
+    }, a.out + static_cast<int64_t>(d.x + r / a.G) * a.o_st + static_cast<int64_t>(d.y * a.G + r % a.G) * a.o_sh);
   pdl_trigger();
 }
 
@@ -1052,41 +1070,16 @@ template <int D, bool F16>
 __global__ void __launch_bounds__(256) paged_tile_join_kernel(const PagedDev a) {
   __shared__ int slot[2 + 8];
   pdl_wait();
-  const int block = blockIdx.y, h = blockIdx.x, lane = threadIdx.x & 31;
+  const int block = blockIdx.y, h = blockIdx.x;
   if (!find_block(a, block, slot, 8)) return;
   const Seq s = seq_of(a, slot[0]);
   const int row0 = slot[1] * kTileRows, rows = min(s.n * a.G - row0, kTileRows);
   const int64_t pitch = static_cast<int64_t>(gridDim.y) * a.HK * kTileRows;
   for (int r = blockIdx.z * 8 + (threadIdx.x >> 5); r < rows; r += 8 * gridDim.z) {
     const int64_t at = (static_cast<int64_t>(block) * a.HK + h) * kTileRows + r;
-    float top = -INFINITY, sum = 0.0f;
-    for (int z = 0; z < a.splits; ++z) top = fmaxf(top, __ldcg(a.ws_ml + at + z * pitch).x);
-    float acc[D / 32];
-#pragma unroll
-    for (int c = 0; c < D / 32; ++c) acc[c] = 0.0f;
-#pragma unroll 4
-    for (int z = 0; z < a.splits; ++z) {
-      const float2 ml = __ldcg(a.ws_ml + at + z * pitch);
-      const float f = ml.x == -INFINITY ? 0.0f : ex2(ml.x - top);
-      sum = fmaf(ml.y, f, sum);
-      const float* src = a.ws_o + (at + z * pitch) * D;
-      if (D == 128) {
-        const float4 v = __ldcg(reinterpret_cast<const float4*>(src) + lane);
-        acc[0] = fmaf(v.x, f, acc[0]), acc[1] = fmaf(v.y, f, acc[1]);
-        acc[2] = fmaf(v.z, f, acc[2]), acc[3] = fmaf(v.w, f, acc[3]);
-      } else {
-        const float2 v = __ldcg(reinterpret_cast<const float2*>(src) + lane);
-        acc[0] = fmaf(v.x, f, acc[0]), acc[1] = fmaf(v.y, f, acc[1]);
-      }
-    }
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    const int pr = row0 + r, j = pr / a.G, hq = h * a.G + pr % a.G;
-    uint16_t* dst = a.out + static_cast<int64_t>(s.q0 + j) * a.o_st + static_cast<int64_t>(hq) * a.o_sh;
-    if (D == 128)
-      reinterpret_cast<uint2*>(dst)[lane] =
-          make_uint2(pack16<F16>(acc[0] * inv, acc[1] * inv), pack16<F16>(acc[2] * inv, acc[3] * inv));
-    else
-      reinterpret_cast<uint32_t*>(dst)[lane] = pack16<F16>(acc[0] * inv, acc[1] * inv);
+    const int pr = row0 + r;
+    join_row<D, F16>(a, a.splits, [&](int z) { return at + z * pitch; },
+                     a.out + static_cast<int64_t>(s.q0 + pr / a.G) * a.o_st + static_cast<int64_t>(h * a.G + pr % a.G) * a.o_sh);
   }
   pdl_trigger();
 }
@@ -1191,7 +1184,7 @@ static cudaError_t launch_split(const CUtensorMap& tk, const CUtensorMap& tv, co
   if (e != cudaSuccess) return e;
   e = launch_kernel(paged_split_kernel<D, MT, F16>, dim3(ctas), dim3(Sh::kThreads), Sh::kBytes, st, true, tk, tv, d);
   if (e != cudaSuccess || d.unit_mode) return e;
-  return launch_kernel(paged_split_join_kernel<D, F16>, dim3(ctas), dim3(512), 0, st, true, d, MT * 16);
+  return launch_kernel(paged_split_join_kernel<D, F16>, dim3(ctas, MT * 4), dim3(128), 0, st, true, d, MT * 16);
 }
 template <int D, bool F16>
 static cudaError_t launch_paged(const qik_paged_attn_args& A, const PagedPlan& p, PagedDev d, uint8_t* ws,
