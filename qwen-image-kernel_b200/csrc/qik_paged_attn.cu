@@ -19,15 +19,15 @@
 //   ragged batches and a single long sequence fill the GPU alike; every CTA finds its
 //   range from the lengths on the device (the host needs none of them, a captured graph
 //   follows them).  A (sequence, head) that one CTA covers is finished there; pieces go
-//   to a workspace and are joined by paged_split_join_kernel in a fixed order.  A TMA
-//   warp fills a ring of K/V tiles; 4 or 8 warps split the tile's keys (and 16-row
-//   groups) between them and run mma.sync m16n8k16: tcgen05's 128-row tiles would be
+//   to a workspace and are joined by paged_split_join_kernel in a fixed order.  Two
+//   TMA warps fill a ring of K and V tiles; 8 warps split the tiles, their keys and the
+//   16-row groups between them and run mma.sync m16n8k16: tcgen05's 128-row tiles would be
 //   8 to 87% padding here and the tensor pipe is not what bounds it.
 //
 //   paged_tile_kernel (more rows: chunks and prompts).  Bound by the tensor core: two
 //   128-row query tiles on tcgen05 share every 128-key tile, as in qik_attn.cu.
 //
-// Pages are fetched by TMA through a 4-D map (D, place, head, page): an index outside the
+// Pages are fetched by TMA through a 5-D map (columns, place, half, head, page): an index outside the
 // pool reads zeros, so a bad page table cannot fault; it is reported in the status word.
 // V rows that no row of the tile sees (behind the last token, before the window) are
 // zeroed in shared memory before the product: whatever an unused place of a page holds,
@@ -106,20 +106,24 @@ __device__ __forceinline__ int tile_at(const Tiles& t, int u) { return u < t.sin
 // ============================================================ few rows: split over keys
 constexpr int kSplitTile = 64;
 
-template <int D, int MT>
+// MT: 16-row groups; TEAMS: sets of warps that take turns at the tiles.  Up to 16 rows the CTA is
+// small and two share an SM, so that one loads while the other changes sequence (the 64 x 500
+// to 12000 keys decode step: 219 us; one CTA of twice the warps and stages: 233 to 245).  With
+// fewer short units than SMs nothing is there to share with: two teams halve the time from
+// tile to tile (one token over 300 keys: 8.1 -> 7.1 us).
+template <int D, int MT, int TEAMS>
 struct SplitShape {
-  static constexpr int kGroups = MT == 4 ? 2 : 4;                 // key groups of a tile
-  static constexpr int kWarps = MT * kGroups;                     // one warp: 16 rows x one key group
-  static constexpr int kKeys = kSplitTile / kGroups;              // keys of a warp in a tile
-  static constexpr int kThreads = (kWarps + 1) * 32;
-  static constexpr int kCtasPerSm = MT == 1 ? 2 : 1;
-  static constexpr int kHalf = kSplitTile * 128;                  // 64 columns of a K or V tile
-  static constexpr int kTileBytes = kHalf * (D / 64);
-  static constexpr int kStages = (MT == 1 ? 3 : 5) * (128 / D);
-  static constexpr int kMergeCols = 32;
-  static constexpr int kMergePitch = kMergeCols + 4;
+  static constexpr int kCtasPerSm = MT == 1 && TEAMS == 1 ? 2 : 1;
+  static constexpr int kWarps = MT == 1 ? 4 * TEAMS : 8;
+  static constexpr int kTeams = TEAMS;
+  static constexpr int kGroups = kWarps / MT;                     // key groups, of all teams
+  static constexpr int kKeys = kSplitTile * kTeams / kGroups;     // keys of a warp in a tile (and 16 rows)
+  static constexpr int kThreads = (kWarps + 2) * 32;              // consumers, K and V producers
+  static constexpr int kTileBytes = kSplitTile * D * 2;           // a K or V tile
+  static constexpr int kStages = 6 / kCtasPerSm * (128 / D);
+  static constexpr int kMergePitch = D + 4;
   static constexpr int kMerge = kStages * 2 * kTileBytes;
-  static constexpr int kMl = kMerge + kGroups * MT * 16 * kMergePitch * 4;
+  static constexpr int kMl = kMerge + (kGroups - 1) * MT * 8 * kMergePitch * 4;
   static constexpr int kBar = kMl + kGroups * MT * 16 * 8;
   static constexpr int kBytes = kBar + 2 * kStages * 8 + 128 + 1024;
   static_assert(kBytes * kCtasPerSm + 1024 * kCtasPerSm <= 233472, "shared memory above an SM's 228 KB");
@@ -153,12 +157,12 @@ __device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t addr) {
 template <bool F16>
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   if (F16)
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
                  "{%0, %1, %2, %3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   else
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
                  "{%0, %1, %2, %3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -184,7 +188,7 @@ struct Walk {
   Seq s;
   Tiles t;
   int i, h, at, nt;      // sequence, head, tile within the unit, the unit's tiles
-  long long left;        // tiles left in the range
+  int left;              // tiles left in the range
 };
 __device__ __forceinline__ bool walk_open(const PagedDev& a, Walk& w) {  // the unit at (i, h); skips empty sequences
   while (w.i < a.B) {
@@ -207,40 +211,37 @@ __device__ __forceinline__ bool walk_next(const PagedDev& a, Walk& w, int taken)
   return walk_open(a, w);
 }
 
-template <int D, int MT, bool F16>
-__global__ void __launch_bounds__(SplitShape<D, MT>::kThreads, SplitShape<D, MT>::kCtasPerSm)
+template <int D, int MT, int TEAMS, bool F16>
+__global__ void __launch_bounds__(SplitShape<D, MT, TEAMS>::kThreads, SplitShape<D, MT, TEAMS>::kCtasPerSm)
     paged_split_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                        const PagedDev a) {
-  using Sh = SplitShape<D, MT>;
+  using Sh = SplitShape<D, MT, TEAMS>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + Sh::kBar);
   uint64_t* empty = full + Sh::kStages;
   volatile int* abort_flag = reinterpret_cast<volatile int*>(empty + Sh::kStages);
-  long long* scan = reinterpret_cast<long long*>(smem + Sh::kMerge);  // before the merge buffer is used
+  volatile int* scan = reinterpret_cast<volatile int*>(smem + Sh::kMerge);  // before the merge buffer is used
   volatile int* found = reinterpret_cast<volatile int*>(smem + Sh::kMl);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int s = 0; s < Sh::kStages; ++s) {
-      mbar_init(&full[s], 1);
-      mbar_init(&empty[s], Sh::kWarps);
+      mbar_init(&full[s], 2);  // the K and the V producer
+      mbar_init(&empty[s], Sh::kWarps / Sh::kTeams);
     }
     *abort_flag = 0;
     found[0] = a.B;
     fence_mbar_init();
   }
-  if (threadIdx.x == 32 * Sh::kWarps) {
-    tma_prefetch_desc(&tm_k);
-    tma_prefetch_desc(&tm_v);
-  }
+  if (warp >= Sh::kWarps && lane == 0) tma_prefetch_desc(warp == Sh::kWarps ? &tm_k : &tm_v);
   pdl_wait();
   __syncthreads();
   if (blockIdx.x == 0) report_bad_lengths(a);
 
   // ---- this CTA's range of tiles
   Walk w;
-  long long share = 0;
+  int share = 0;
   if (a.unit_mode) {
     w.i = blockIdx.x / a.HK;
     w.h = blockIdx.x % a.HK;
@@ -250,39 +251,51 @@ __global__ void __launch_bounds__(SplitShape<D, MT>::kThreads, SplitShape<D, MT>
   } else {
     Seq s;
     Tiles t;
-    long long sum = 0;
-    for (int i = threadIdx.x; i < a.B; i += Sh::kThreads) sum += static_cast<long long>(split_tiles(a, i, s, t)) * a.HK;
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (lane == 0) scan[warp] = sum;
-    __syncthreads();
-    long long total = 0;
-    for (int k = 0; k <= Sh::kWarps; ++k) total += scan[k];
-    share = max(static_cast<long long>(a.min_share), (total + gridDim.x - 1) / gridDim.x);
-    const long long begin = share * blockIdx.x;
-    w.left = min(share, total - begin);
+    int mine = 0, sum = 0;
+    for (int i = threadIdx.x; i < a.B; i += Sh::kThreads) {
+      mine = split_tiles(a, i, s, t) * a.HK;
+      sum += mine;
+    }
+    // what the threads before this one hold, and all of them
+    auto scan_block = [&](int v, int& total) {
+      int incl = v;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int up = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += up;
+      }
+      if (lane == 31) scan[warp] = incl;
+      __syncthreads();
+      total = 0;
+#pragma unroll
+      for (int k = 0; k < Sh::kThreads / 32; ++k) {
+        if (k == warp) incl += total;
+        total += scan[k];
+      }
+      return incl - v;
+    };
+    int total, excl = scan_block(sum, total);
+    share = max(a.min_share, static_cast<int>((static_cast<uint32_t>(total) + gridDim.x - 1) / gridDim.x));
+    const long long begin = static_cast<long long>(share) * blockIdx.x;
+    w.left = static_cast<int>(min(static_cast<long long>(share), total - begin));
     if (w.left > 0) {  // uniform over the CTA: find the sequence that holds tile `begin`
-      long long base = 0;
+      const int want = static_cast<int>(begin);
+      int base = 0;
       for (int i0 = 0; i0 < a.B; i0 += Sh::kThreads) {
         const int i = i0 + threadIdx.x;
-        const long long mine = i < a.B ? static_cast<long long>(split_tiles(a, i, s, t)) * a.HK : 0;
-        long long incl = mine;
-        for (int o = 1; o < 32; o <<= 1) {
-          const long long up = __shfl_up_sync(0xffffffffu, incl, o);
-          if (lane >= o) incl += up;
+        if (a.B > Sh::kThreads) {
+          mine = i < a.B ? split_tiles(a, i, s, t) * a.HK : 0;
+          __syncthreads();  // the last sums have been read
+          excl = base + scan_block(mine, total);
+          base += total;
         }
-        __syncthreads();
-        if (lane == 31) scan[warp] = incl;
-        __syncthreads();
-        for (int k = 0; k < warp; ++k) incl += scan[k];
-        const long long excl = base + incl - mine;
-        if (mine > 0 && excl <= begin && begin < excl + mine) {
-          const int nt = static_cast<int>(mine / a.HK);
-          found[1] = static_cast<int>((begin - excl) / nt);
-          found[2] = static_cast<int>((begin - excl) % nt);
+        if (mine > 0 && excl <= want && want < excl + mine) {
+          const int nt = mine / a.HK, rest = want - excl;
+          found[1] = rest / nt;
+          found[2] = rest % nt;
           found[0] = i;
         }
-        for (int k = 0; k <= Sh::kWarps; ++k) base += scan[k];
-        if (base > begin) break;
+        if (base > want) break;
       }
       __syncthreads();
       w.i = found[0];
@@ -302,54 +315,52 @@ __global__ void __launch_bounds__(SplitShape<D, MT>::kThreads, SplitShape<D, MT>
   auto k_ptr = [&](int s) { return smem + s * 2 * Sh::kTileBytes; };
   auto v_ptr = [&](int s) { return smem + s * 2 * Sh::kTileBytes + Sh::kTileBytes; };
 
-  if (warp == Sh::kWarps) {
-    // ------------------------------------------------------------ producer
-    const int page = 1 << a.page_log2;
-    const int box = min(page, kSplitTile);
-    const int pieces = kSplitTile / box;
+  const int box_log2 = min(a.page_log2, 6);  // tokens of one TMA piece: a page's share of a tile
+  static_assert(kSplitTile == 64, "pieces of 2^box_log2 tokens");
+  if (warp >= Sh::kWarps) {
+    // ------------------------------------------------------------ producers (K, V)
+    const bool is_k = warp == Sh::kWarps;
+    const CUtensorMap* tm = is_k ? &tm_k : &tm_v;
+    const int pieces_log2 = 6 - box_log2, pieces = 1 << pieces_log2;
+    const int piece = lane & (pieces - 1);
+    const int run = 32 >> pieces_log2;  // tiles whose page numbers one load of the warp brings
     int stage = 0;
     uint32_t phase = 1;
     bool more = true, ok = true;
     while (more && ok) {
-      const int count = static_cast<int>(min(static_cast<long long>(w.nt - w.at), w.left));
+      const int count = min(w.nt - w.at, w.left);
       const int32_t* row = a.table + static_cast<int64_t>(w.i) * a.table_st;
-      // lane's page number for its piece of the tiles [u, u + 32 / pieces): one load serves them
-      // all, and the next is in flight while they are issued.  Behind the last token (or
-      // outside the table) there is none, which reads as zeros like any page outside the pool
+      // lane's page number for its piece of tile u0 + lane / pieces: one load serves `run` tiles,
+      // and the next is in flight while they are issued.  Behind the last token (or outside
+      // the table) there is none, which reads as zeros like any page outside the pool
       auto page_of = [&](int u0) {
-        const int u = u0 + lane / pieces;
+        const int u = u0 + (lane >> pieces_log2);
         if (u >= w.at + count || w.t.main == 0) return -1;
-        const int key = tile_at(w.t, u) * kSplitTile + (lane % pieces) * box;
+        const int key = tile_at(w.t, u) * kSplitTile + (piece << box_log2);
         const int p = key >> a.page_log2;
         if (key >= w.s.kv || p >= a.W) return -1;
         const int id = __ldg(row + p);
         if ((id < 0 || id >= a.pages) && a.status) atomicExch(a.status, QIK_DEV_BAD_INDEX);
         return id < a.pages ? id : -1;
       };
-      const int run = 32 / pieces;  // tiles that one load serves
       int cur = 0, next = page_of(w.at);
       for (int u = w.at; u < w.at + count; ++u) {
-        const int k = (u - w.at) % run;
+        const int k = (u - w.at) & (run - 1);
         if (k == 0) {
           cur = next;
           next = page_of(u + run);
         }
-        const int id = __shfl_sync(0xffffffffu, cur, k * pieces + lane % pieces);
+        const int id = __shfl_sync(0xffffffffu, cur, (k << pieces_log2) + piece);
         if (!__all_sync(0xffffffffu, mbar_wait(&empty[stage], phase, abort_flag, a.status))) {
           ok = false;
           break;
         }
-        if (lane == 0) mbar_arrive_expect_tx(&full[stage], 2 * Sh::kTileBytes);
+        if (lane == 0) mbar_arrive_expect_tx(&full[stage], Sh::kTileBytes);
         __syncwarp();
-        if (lane < pieces) {
-          const int place = (tile_at(w.t, u) * kSplitTile + lane * box) & (page - 1);
-#pragma unroll
-          for (int hd = 0; hd < D / 64; ++hd) {
-            const int off = hd * Sh::kHalf + lane * box * 128;
-            tma_load_4d(k_ptr(stage) + off, &tm_k, hd * 64, place, w.h, id, &full[stage]);
-            tma_load_4d(v_ptr(stage) + off, &tm_v, hd * 64, place, w.h, id, &full[stage]);
-          }
-        }
+        if (lane < pieces)
+          tma_load_5d((is_k ? k_ptr(stage) : v_ptr(stage)) + (piece << box_log2) * (D * 2), tm, 0,
+                      (tile_at(w.t, u) * kSplitTile + (piece << box_log2)) & ((1 << a.page_log2) - 1), 0, w.h, id,
+                      &full[stage]);
         if (++stage == Sh::kStages) stage = 0, phase ^= 1u;
       }
       more = walk_next(a, w, count);
@@ -357,12 +368,21 @@ __global__ void __launch_bounds__(SplitShape<D, MT>::kThreads, SplitShape<D, MT>
   } else {
     // ------------------------------------------------------------ consumers
     const int mt = warp % MT, kg = warp / MT;
+    const int team = kg * Sh::kTeams / Sh::kGroups;  // the tiles that this warp takes: every kTeams-th
+    const int key0 = kg % (Sh::kGroups / Sh::kTeams) * Sh::kKeys;  // its first key in them
+    int turn = 0;
     const int g = lane >> 2, c2 = (lane & 3) * 2;
+    // byte of the 16-byte chunk ch of a key in a tile: pieces of 2^box_log2 keys, each as halves of
+    // 64 columns in 128-byte-swizzled rows (a 16-key block never crosses a piece)
+    auto place = [&](int key, int ch) {
+      const int in = key & ((1 << box_log2) - 1);
+      return (key - in) * (D * 2) + ((ch >> 3) << (box_log2 + 7)) + in * 128 + (((ch & 7) ^ (key & 7)) << 4);
+    };
     int stage = 0;
     uint32_t phase = 0;
     bool more = true, ok = true;
     while (more && ok) {
-      const int count = static_cast<int>(min(static_cast<long long>(w.nt - w.at), w.left));
+      const int count = min(w.nt - w.at, w.left);
       const int rows = w.s.n * a.G;
       const bool mine = mt * 16 < rows;
       // this lane's two rows: token, limits; q fragments straight from global memory
@@ -392,44 +412,65 @@ __global__ void __launch_bounds__(SplitShape<D, MT>::kThreads, SplitShape<D, MT>
 
       for (int u = w.at; u < w.at + count; ++u) {
         const int kv0 = tile_at(w.t, u) * kSplitTile;
+        if (Sh::kTeams > 1 && (turn++ & 1) != team) {
+          if (++stage == Sh::kStages) stage = 0, phase ^= 1u;
+          continue;
+        }
         if (!__all_sync(0xffffffffu, mbar_wait(&full[stage], phase, abort_flag, a.status))) {
           ok = false;
           break;
         }
         if (mine) {
           const uint32_t kb = smem_u32(k_ptr(stage)), vb = smem_u32(v_ptr(stage));
-          const int key0 = kg * Sh::kKeys;  // this warp's first key of the tile
           // V rows that no row sees (see the top of the file)
           const bool edge = kv0 + kSplitTile - 1 > w.t.lmax || (kv0 < w.t.lmin && kv0 + kSplitTile - 1 >= a.sinks);
           if (edge) {
             for (int x = lane; x < Sh::kKeys * (D / 8); x += 32) {
               const int key = key0 + x / (D / 8), ch = x % (D / 8), kv = kv0 + key;
               if (kv > w.t.lmax || (kv < w.t.lmin && kv >= a.sinks))
-                *reinterpret_cast<uint4*>(v_ptr(stage) + (ch >> 3) * Sh::kHalf + key * 128 + ((ch & 7) << 4 ^ (key & 7) << 4)) =
-                    make_uint4(0u, 0u, 0u, 0u);
+                *reinterpret_cast<uint4*>(v_ptr(stage) + place(key, ch)) = make_uint4(0u, 0u, 0u, 0u);
             }
             fence_proxy_async_smem();  // before the next TMA write of this stage
             __syncwarp();
           }
-          // S = Q K^T for kKeys keys
+          // S = Q K^T for kKeys keys: a 16-key block's fragments are loaded back to back (one
+          // shared-memory latency a block), then multiplied in chains of D / 32 products
           float s[Sh::kKeys / 8][4];
 #pragma unroll
-          for (int n = 0; n < Sh::kKeys / 8; ++n)
+          for (int n2 = 0; n2 < Sh::kKeys / 16; ++n2) {
+            constexpr int kBatch = MT == 1 ? D / 16 : 4;
+            float odd[2][4];
 #pragma unroll
-            for (int c = 0; c < 4; ++c) s[n][c] = 0.0f;
+            for (int c = 0; c < 4; ++c) s[2 * n2][c] = s[2 * n2 + 1][c] = odd[0][c] = odd[1][c] = 0.0f;
 #pragma unroll
-          for (int k = 0; k < D / 16; ++k) {
+            for (int k0 = 0; k0 < D / 16; k0 += kBatch) {
+              uint32_t kf[kBatch][4];
 #pragma unroll
-            for (int n2 = 0; n2 < Sh::kKeys / 16; ++n2) {
-              const int mat = lane >> 3;
-              const int key = key0 + n2 * 16 + (mat >> 1) * 8 + (lane & 7);
-              const int ch = k * 2 + (mat & 1);
-              uint32_t b[4];
-              ldsm4(b, kb + (ch >> 3) * Sh::kHalf + key * 128 + (((ch & 7) ^ (key & 7)) << 4));
-              mma16816<F16>(s[2 * n2], qf[k], b[0], b[1]);
-              mma16816<F16>(s[2 * n2 + 1], qf[k], b[2], b[3]);
+              for (int k = 0; k < kBatch; ++k) {
+                const int key = key0 + n2 * 16 + (lane >> 4) * 8 + (lane & 7);
+                ldsm4(kf[k], kb + place(key, (k0 + k) * 2 + ((lane >> 3) & 1)));
+              }
+#pragma unroll
+              for (int k = 0; k < kBatch; k += 2) {
+                mma16816<F16>(s[2 * n2], qf[k0 + k], kf[k][0], kf[k][1]);
+                mma16816<F16>(s[2 * n2 + 1], qf[k0 + k], kf[k][2], kf[k][3]);
+                mma16816<F16>(odd[0], qf[k0 + k + 1], kf[k + 1][0], kf[k + 1][1]);
+                mma16816<F16>(odd[1], qf[k0 + k + 1], kf[k + 1][2], kf[k + 1][3]);
+              }
             }
+#pragma unroll
+            for (int c = 0; c < 4; ++c) s[2 * n2][c] += odd[0][c], s[2 * n2 + 1][c] += odd[1][c];
           }
+          // V fragments of the first 16 keys: in flight during the softmax
+          uint32_t vf[D / 16][4];
+          auto load_v = [&](int k2) {
+#pragma unroll
+            for (int d2 = 0; d2 < D / 16; ++d2) {
+              const int key = key0 + k2 * 16 + ((lane >> 3) & 1) * 8 + (lane & 7);
+              ldsm4_t(vf[d2], vb + place(key, d2 * 2 + (lane >> 4)));
+            }
+          };
+          load_v(0);
           // masks, unless every row sees the whole tile
           const bool whole = kv0 + kSplitTile - 1 <= first_last && (kv0 >= last_first || kv0 + kSplitTile - 1 < a.sinks);
           float mx[2] = {-INFINITY, -INFINITY};
@@ -482,15 +523,11 @@ __global__ void __launch_bounds__(SplitShape<D, MT>::kThreads, SplitShape<D, MT>
           // O += P V
 #pragma unroll
           for (int k2 = 0; k2 < Sh::kKeys / 16; ++k2) {
+            if (k2 > 0) load_v(k2);
 #pragma unroll
             for (int d2 = 0; d2 < D / 16; ++d2) {
-              const int mat = lane >> 3;
-              const int key = key0 + k2 * 16 + (mat & 1) * 8 + (lane & 7);
-              const int ch = d2 * 2 + (mat >> 1);
-              uint32_t b[4];
-              ldsm4_t(b, vb + (ch >> 3) * Sh::kHalf + key * 128 + (((ch & 7) ^ (key & 7)) << 4));
-              mma16816<F16>(o[2 * d2], p[k2], b[0], b[1]);
-              mma16816<F16>(o[2 * d2 + 1], p[k2], b[2], b[3]);
+              mma16816<F16>(o[2 * d2], p[k2], vf[d2][0], vf[d2][1]);
+              mma16816<F16>(o[2 * d2 + 1], p[k2], vf[d2][2], vf[d2][3]);
             }
           }
         }
@@ -501,7 +538,8 @@ __global__ void __launch_bounds__(SplitShape<D, MT>::kThreads, SplitShape<D, MT>
       // a wait that gave up ends the CTA's consumers together
       if (named_bar_any(1, Sh::kWarps * 32, !ok)) break;
 
-      // ---- join the key groups: maxima and sums, then 32 columns at a time
+      // ---- join the key groups: maxima and sums, then 8 of each 16 rows at a time; the first
+      // group's warp adds the others' and stores
       float2* ml = reinterpret_cast<float2*>(smem + Sh::kMl);
       float* mg = reinterpret_cast<float*>(smem + Sh::kMerge);
 #pragma unroll
@@ -511,50 +549,56 @@ __global__ void __launch_bounds__(SplitShape<D, MT>::kThreads, SplitShape<D, MT>
         if ((lane & 3) == 0) ml[kg * MT * 16 + mt * 16 + g + 8 * x] = make_float2(m[x], l[x]);
       }
       named_bar_sync(1, Sh::kWarps * 32);
-      float f[2];
-#pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        float top = -INFINITY;
-        for (int k = 0; k < Sh::kGroups; ++k) top = fmaxf(top, ml[k * MT * 16 + mt * 16 + g + 8 * x].x);
-        f[x] = m[x] == -INFINITY ? 0.0f : ex2(m[x] - top);
-      }
       const bool begins = w.at == 0, ends = w.at + count == w.nt;
       const int slot = 2 * blockIdx.x + (begins ? 1 : 0);
 #pragma unroll
-      for (int cc = 0; cc < D / Sh::kMergeCols; ++cc) {
+      for (int x = 0; x < 2; ++x) {
+        if (x == 1 && rows <= 8) break;
+        const int r = mt * 16 + g + 8 * x;
+        float top = -INFINITY, sum = 0.0f;
 #pragma unroll
-        for (int n = 0; n < 4; ++n)
+        for (int k = 0; k < Sh::kGroups; ++k) top = fmaxf(top, ml[k * MT * 16 + r].x);
 #pragma unroll
-          for (int x = 0; x < 2; ++x)
-            *reinterpret_cast<float2*>(mg + (kg * MT * 16 + mt * 16 + g + 8 * x) * Sh::kMergePitch + n * 8 + c2) =
-                make_float2(o[cc * 4 + n][2 * x] * f[x], o[cc * 4 + n][2 * x + 1] * f[x]);
-        named_bar_sync(1, Sh::kWarps * 32);
-        for (int it = threadIdx.x; it < MT * 16 * 8; it += Sh::kWarps * 32) {
-          const int r = it >> 3, col = (it & 7) * 4;
-          if (r < rows) {
-            float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            float top = -INFINITY, sum = 0.0f;
-            for (int k = 0; k < Sh::kGroups; ++k) top = fmaxf(top, ml[k * MT * 16 + r].x);
-            for (int k = 0; k < Sh::kGroups; ++k) {
-              const float4 t = *reinterpret_cast<const float4*>(mg + (k * MT * 16 + r) * Sh::kMergePitch + col);
-              v.x += t.x, v.y += t.y, v.z += t.z, v.w += t.w;
-              const float2 e = ml[k * MT * 16 + r];
-              sum += e.x == -INFINITY ? 0.0f : e.y * ex2(e.x - top);
-            }
-            if (begins && ends) {
-              const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-              const int j = r / a.G, hq = w.h * a.G + r % a.G;
-              *reinterpret_cast<uint2*>(a.out + static_cast<int64_t>(w.s.q0 + j) * a.o_st +
-                                        static_cast<int64_t>(hq) * a.o_sh + cc * Sh::kMergeCols + col) =
-                  make_uint2(pack16<F16>(v.x * inv, v.y * inv), pack16<F16>(v.z * inv, v.w * inv));
-            } else {
-              const int64_t at = static_cast<int64_t>(slot) * (MT * 16) + r;
-              *reinterpret_cast<float4*>(a.ws_o + at * D + cc * Sh::kMergeCols + col) = v;
-              if (cc == 0 && col == 0) a.ws_ml[at] = make_float2(top, sum);
-            }
-          }
+        for (int k = 0; k < Sh::kGroups; ++k) {
+          const float2 e = ml[k * MT * 16 + r];
+          sum += e.x == -INFINITY ? e.y : e.y * ex2(e.x - top);  // (no key seen: 0, or NaN)
+        }
+        const float f = m[x] == -INFINITY ? 1.0f : ex2(m[x] - top);
+        if (x == 1) named_bar_sync(1, Sh::kWarps * 32);
+        float* part = mg + ((kg - 1) * MT * 8 + mt * 8 + g) * Sh::kMergePitch + c2;
+        if (kg > 0) {
+#pragma unroll
+          for (int n = 0; n < D / 8; ++n)
+            *reinterpret_cast<float2*>(part + n * 8) = make_float2(o[n][2 * x] * f, o[n][2 * x + 1] * f);
         }
         named_bar_sync(1, Sh::kWarps * 32);
+        if (kg == 0) {
+          const float* src = mg + (mt * 8 + g) * Sh::kMergePitch + c2;
+          const bool whole = begins && ends;
+          const float inv = !whole ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum;
+          const int64_t at = static_cast<int64_t>(slot) * (MT * 16) + r;
+          uint16_t* dst = a.out + static_cast<int64_t>(w.s.q0 + r / a.G) * a.o_st +
+                          static_cast<int64_t>(w.h * a.G + r % a.G) * a.o_sh + c2;
+          float v[D / 8][2];
+#pragma unroll
+          for (int n = 0; n < D / 8; ++n) v[n][0] = o[n][2 * x] * f, v[n][1] = o[n][2 * x + 1] * f;
+#pragma unroll
+          for (int k = 0; k < Sh::kGroups - 1; ++k)
+#pragma unroll
+            for (int n = 0; n < D / 8; ++n) {
+              const float2 e = *reinterpret_cast<const float2*>(src + k * MT * 8 * Sh::kMergePitch + n * 8);
+              v[n][0] += e.x, v[n][1] += e.y;
+            }
+          if (r < rows && whole) {
+#pragma unroll
+            for (int n = 0; n < D / 8; ++n) *reinterpret_cast<uint32_t*>(dst + n * 8) = pack16<F16>(v[n][0] * inv, v[n][1] * inv);
+          } else if (r < rows) {
+#pragma unroll
+            for (int n = 0; n < D / 8; ++n)
+              *reinterpret_cast<float2*>(a.ws_o + at * D + n * 8 + c2) = make_float2(v[n][0], v[n][1]);
+          }
+          if (r < rows && !whole && c2 == 0) a.ws_ml[at] = make_float2(top, sum);
+        }
       }
       if (begins && !ends && threadIdx.x == 0)
         a.ws_desc[blockIdx.x] = make_int4(w.s.q0, w.h, static_cast<int>((w.nt - count + share - 1) / share), rows);
@@ -849,7 +893,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         const int place = (kv_of(t) + lane * box) & (page - 1);
 #pragma unroll
         for (int hd = 0; hd < Sh::kHalves; ++hd)
-          tma_load_4d(dst + hd * Sh::kHalfBytes + lane * box * 128, tm, hd * 64, place, h, id, bar);
+          tma_load_5d(dst + hd * Sh::kHalfBytes + lane * box * 128, tm, 0, place, hd, h, id, bar);
       }
     };
     // step u: K of tile u, then V of tile u - 1
@@ -1109,7 +1153,7 @@ static PagedPlan paged_plan(const qik_paged_attn_args& A) {
   if (p.split) {
     p.split_mt = max_rows <= 16 ? 1 : max_rows <= 32 ? 2 : 4;
     // short contexts (at most 8 tiles): one CTA for each (sequence, head), nothing to join
-    p.unit_mode = A.max_kv <= 8 * kSplitTile && A.B * A.HK <= 0x7FFFFFFFll;
+    p.unit_mode = A.max_kv <= 8 * kSplitTile;
     p.split_ctas = p.unit_mode ? static_cast<int>(A.B * A.HK) : sms * (p.split_mt == 1 ? 2 : 1);
     if (!p.unit_mode) {
       const size_t rows = static_cast<size_t>(2) * p.split_ctas * p.split_mt * 16;
@@ -1146,6 +1190,9 @@ static int check_paged(const qik_paged_attn_args& A) {
               "qik_paged_attention: page of %lld tokens (a power of two, 16 to 4096), %lld pages", (long long)A.page,
               (long long)A.pages);
   QIK_REQUIRE(A.W >= 0 && A.W * A.page <= (1ll << 30), "qik_paged_attention: page table of %lld columns", (long long)A.W);
+  QIK_REQUIRE(A.B * A.HK <= 0x7FFFFFFFll && A.B * A.HK * (A.W * A.page / kSplitTile + 3) <= 0x7FFFFFFFll,
+              "qik_paged_attention: %lld sequences of up to %lld keys are too much for one call", (long long)A.B,
+              (long long)(A.W * A.page));
   QIK_REQUIRE(A.max_new >= 0 && A.max_new <= A.T && A.max_kv >= 0, "qik_paged_attention: max_new %lld of %lld tokens, max_kv %lld",
               (long long)A.max_new, (long long)A.T, (long long)A.max_kv);
   QIK_REQUIRE(A.window >= 0 && A.sinks >= 0 && A.window <= 0x3FFFFFFF && A.sinks <= 0x3FFFFFFF,
@@ -1155,13 +1202,16 @@ static int check_paged(const qik_paged_attn_args& A) {
   return QIK_OK;
 }
 
+// (64 columns, place, 64-column half, head, page): one load brings a piece's halves one after
+// the other; `halves` of them (the tile kernel's operands want them 128 rows apart and load
+// them one by one).
 static int page_map(CUtensorMap* m, const void* base, bool f16, const qik_paged_attn_args& A, int64_t s0, int64_t sh,
-                    int64_t ss, int64_t tile) {
-  const uint64_t dims[4] = {static_cast<uint64_t>(A.D), static_cast<uint64_t>(A.page), static_cast<uint64_t>(A.HK),
+                    int64_t ss, int64_t tile, uint32_t halves) {
+  const uint64_t dims[5] = {64, static_cast<uint64_t>(A.page), static_cast<uint64_t>(A.D / 64), static_cast<uint64_t>(A.HK),
                             static_cast<uint64_t>(A.pages)};
-  const uint64_t strides[3] = {static_cast<uint64_t>(ss * 2), static_cast<uint64_t>(sh * 2), static_cast<uint64_t>(s0 * 2)};
-  const uint32_t box[4] = {64, static_cast<uint32_t>(A.page < tile ? A.page : tile), 1, 1};
-  return make_tmap_nd(m, base, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, dims,
+  const uint64_t strides[4] = {static_cast<uint64_t>(ss * 2), 128, static_cast<uint64_t>(sh * 2), static_cast<uint64_t>(s0 * 2)};
+  const uint32_t box[5] = {64, static_cast<uint32_t>(A.page < tile ? A.page : tile), halves, 1, 1};
+  return make_tmap_nd(m, base, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5, dims,
                       strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
@@ -1176,13 +1226,13 @@ static cudaError_t allow_smem(K kernel, int bytes, std::once_flag* once) {
   return e;
 }
 
-template <int D, int MT, bool F16>
+template <int D, int MT, int TEAMS, bool F16>
 static cudaError_t launch_split(const CUtensorMap& tk, const CUtensorMap& tv, const PagedDev& d, int ctas, cudaStream_t st) {
-  using Sh = SplitShape<D, MT>;
+  using Sh = SplitShape<D, MT, TEAMS>;
   static std::once_flag once[64];
-  cudaError_t e = allow_smem(paged_split_kernel<D, MT, F16>, Sh::kBytes, once);
+  cudaError_t e = allow_smem(paged_split_kernel<D, MT, TEAMS, F16>, Sh::kBytes, once);
   if (e != cudaSuccess) return e;
-  e = launch_kernel(paged_split_kernel<D, MT, F16>, dim3(ctas), dim3(Sh::kThreads), Sh::kBytes, st, true, tk, tv, d);
+  e = launch_kernel(paged_split_kernel<D, MT, TEAMS, F16>, dim3(ctas), dim3(Sh::kThreads), Sh::kBytes, st, true, tk, tv, d);
   if (e != cudaSuccess || d.unit_mode) return e;
   return launch_kernel(paged_split_join_kernel<D, F16>, dim3(ctas, MT * 4), dim3(128), 0, st, true, d, MT * 16);
 }
@@ -1198,9 +1248,11 @@ static cudaError_t launch_paged(const qik_paged_attn_args& A, const PagedPlan& p
     s.ws_o = reinterpret_cast<float*>(ws + p.split_o);
     s.ws_ml = reinterpret_cast<float2*>(ws + p.split_ml);
     s.ws_desc = reinterpret_cast<int4*>(ws + p.split_desc);
-    e = p.split_mt == 1   ? launch_split<D, 1, F16>(maps[0], maps[1], s, p.split_ctas, st)
-        : p.split_mt == 2 ? launch_split<D, 2, F16>(maps[0], maps[1], s, p.split_ctas, st)
-                          : launch_split<D, 4, F16>(maps[0], maps[1], s, p.split_ctas, st);
+    const bool few = p.unit_mode && p.split_ctas <= sm_count();
+    e = p.split_mt == 1   ? (few ? launch_split<D, 1, 2, F16>(maps[0], maps[1], s, p.split_ctas, st)
+                                 : launch_split<D, 1, 1, F16>(maps[0], maps[1], s, p.split_ctas, st))
+        : p.split_mt == 2 ? launch_split<D, 2, 1, F16>(maps[0], maps[1], s, p.split_ctas, st)
+                          : launch_split<D, 4, 1, F16>(maps[0], maps[1], s, p.split_ctas, st);
     if (e != cudaSuccess) return e;
   }
   if (p.tile) {
@@ -1251,12 +1303,12 @@ extern "C" int qik_paged_attention(const qik_paged_attn_args* args, void* ws, si
   const bool f16 = (A.flags & QIK_PAGED_F16) != 0;
   CUtensorMap maps[4];
   if (p.split) {
-    rc = page_map(&maps[0], A.k_pages, f16, A, A.kp_s0, A.kp_sh, A.kp_ss, kSplitTile);
-    if (!rc) rc = page_map(&maps[1], A.v_pages, f16, A, A.vp_s0, A.vp_sh, A.vp_ss, kSplitTile);
+    rc = page_map(&maps[0], A.k_pages, f16, A, A.kp_s0, A.kp_sh, A.kp_ss, kSplitTile, static_cast<uint32_t>(A.D / 64));
+    if (!rc) rc = page_map(&maps[1], A.v_pages, f16, A, A.vp_s0, A.vp_sh, A.vp_ss, kSplitTile, static_cast<uint32_t>(A.D / 64));
   }
   if (!rc && p.tile) {
-    rc = page_map(&maps[2], A.k_pages, f16, A, A.kp_s0, A.kp_sh, A.kp_ss, kTileN);
-    if (!rc) rc = page_map(&maps[3], A.v_pages, f16, A, A.vp_s0, A.vp_sh, A.vp_ss, kTileN);
+    rc = page_map(&maps[2], A.k_pages, f16, A, A.kp_s0, A.kp_sh, A.kp_ss, kTileN, 1);
+    if (!rc) rc = page_map(&maps[3], A.v_pages, f16, A, A.vp_s0, A.vp_sh, A.vp_ss, kTileN, 1);
   }
   if (rc) return rc;
   PagedDev d = {};

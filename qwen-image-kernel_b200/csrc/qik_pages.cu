@@ -16,8 +16,8 @@
 
 namespace qik {
 
-constexpr int kPageThreads = 128;
-constexpr int kPageUnroll = 4;
+constexpr int kPageThreads = 32;
+constexpr int kPageUnroll = 16;
 
 template <int N>
 struct PageMoves {
@@ -31,7 +31,10 @@ struct PagePools {
   int token_bytes, heads, layers, page;
 };
 
-// blockIdx.x: (pool, layer, head); blockIdx.y: move; blockIdx.z: 8 KB of the run.
+// blockIdx.x: (pool, layer, head); blockIdx.y: move; blockIdx.z: 8 KB of the run.  Sixteen loads in flight a
+// thread and many small CTAs: 500 whole pages (3.1 GB moved) 506 us with 32 threads x 16, 513 with
+// 64 x 16, 535 with 128 x 8, 579 with 128 x 4; bulk copies through shared memory 547 (and 22.5
+// instead of 6.8 us for seven partly filled pages).
 template <int N>
 __global__ void __launch_bounds__(kPageThreads) copy_pages_kernel(const __grid_constant__ PageMoves<N> m,
                                                                   const PagePools p) {
@@ -124,7 +127,7 @@ extern "C" int qik_copy_pages(const qik_page_pools* pools, const int32_t* moves,
   p.head_bytes[0] = A.k_head_bytes, p.head_bytes[1] = A.v_head_bytes;
   p.token_bytes = static_cast<int>(A.token_bytes), p.heads = static_cast<int>(A.heads);
   p.layers = static_cast<int>(A.layers), p.page = static_cast<int>(A.page);
-  // one CTA for each 8 KB of a head's run (4 vectors a thread)
+  // one CTA of one warp for each 8 KB of a head's run (16 vectors a thread)
   const int64_t chunk = kPageThreads * kPageUnroll * 16;
   const int64_t chunks = (most * A.token_bytes + chunk - 1) / chunk;
   const int z = static_cast<int>(chunks < 65535 ? chunks : 65535);

@@ -55,8 +55,11 @@ __device__ __forceinline__ int64_t load_index(const void* p, int64_t i, bool wid
   return wide ? __ldg(static_cast<const long long*>(p) + i) : static_cast<int64_t>(__ldg(static_cast<const int*>(p) + i));
 }
 
-// ITEMS = D / 16 lanes a head: lane item i holds pairs 8i .. 8i + 7 of the rotated part
-// (i < rot / 16) or 16 of the copied columns.
+// ITEMS = D / 16 lanes a head, two 16-byte vectors each, laid so that neighbouring lanes read
+// neighbouring vectors.  Streaming loads and stores: 8111 tokens of 72 heads (301 MB) take 49.9 us
+// (6.04 TB/s), 55.0 without the hints.
+// Halves: lane item i < rot / 16 holds columns 8i .. 8i + 7 and their partners rot / 2 on, the
+// others the copied columns.  Interleaved: columns 8i .. and D / 2 + 8i .., either turned or not.
 template <bool F16, int ITEMS>
 __global__ void __launch_bounds__(kRotaryWarps * 32) rotary_kernel(const RotaryDev a) {
   constexpr int kHeadsPerStep = 32 / ITEMS;
@@ -68,11 +71,22 @@ __global__ void __launch_bounds__(kRotaryWarps * 32) rotary_kernel(const RotaryD
   const int item = lane % ITEMS;
   const int head0 = static_cast<int>(task % a.tasks_per_token) * (kHeadsPerStep * kRotarySteps) + lane / ITEMS;
   const int heads = a.HQ + a.HK + a.HV;
-  const bool turned = item < a.rot / 16;
-  // the two vectors of this lane: columns of the first and of the second
   const int half = a.rot / 2;
-  const int c0 = turned && !a.interleaved ? 8 * item : 16 * item;
-  const int c1 = turned && !a.interleaved ? half + 8 * item : 16 * item + 8;
+  const int turned_items = a.rot / 16;
+  int c0 = 8 * item, c1;  // first columns of the two vectors
+  bool t0, t1;            // turned
+  if (a.interleaved) {
+    c1 = a.D / 2 + c0;
+    t0 = c0 < a.rot;
+    t1 = c1 < a.rot;
+  } else {
+    t0 = t1 = item < turned_items;
+    c1 = c0 + half;
+    if (!t0) {
+      c0 = a.rot + 8 * (item - turned_items);
+      c1 = c0 + (a.D - a.rot) / 2;
+    }
+  }
 
   const int64_t pos = load_index(a.positions, t, a.pos64);
   const bool pos_ok = pos >= 0 && pos < a.P;
@@ -95,20 +109,25 @@ __global__ void __launch_bounds__(kRotaryWarps * 32) rotary_kernel(const RotaryD
       const uint16_t* src = hd < a.HQ            ? a.q + t * a.q_st + hd * a.q_sh
                             : hd < a.HQ + a.HK ? a.k + t * a.k_st + (hd - a.HQ) * a.k_sh
                                                  : a.v + t * a.v_st + (hd - a.HQ - a.HK) * a.v_sh;
-      v0[s] = __ldg(reinterpret_cast<const uint4*>(src + c0));
-      v1[s] = __ldg(reinterpret_cast<const uint4*>(src + c1));
+      v0[s] = __ldcs(reinterpret_cast<const uint4*>(src + c0));
+      v1[s] = __ldcs(reinterpret_cast<const uint4*>(src + c1));
     }
   }
+  // eight angles: those of the 8 pairs (halves), or of the 4 pairs of each vector
   float c[8], sn[8];
-  if (turned && pos_ok) {
-    const float4* cp = reinterpret_cast<const float4*>(a.cos + pos * half + 8 * item);
-    const float4* sp = reinterpret_cast<const float4*>(a.sin + pos * half + 8 * item);
-    const float4 ca = __ldg(cp), cb = __ldg(cp + 1), sa = __ldg(sp), sb = __ldg(sp + 1);
+  {
+    const int p0 = a.interleaved ? c0 / 2 : c0, p1 = a.interleaved ? c1 / 2 : c0 + 4;
+    float4 ca = make_float4(1.0f, 1.0f, 1.0f, 1.0f), sa = make_float4(0.0f, 0.0f, 0.0f, 0.0f), cb = ca, sb = sa;
+    if (t0 && pos_ok) {
+      ca = __ldg(reinterpret_cast<const float4*>(a.cos + pos * half + p0));
+      sa = __ldg(reinterpret_cast<const float4*>(a.sin + pos * half + p0));
+    }
+    if (t1 && pos_ok) {
+      cb = __ldg(reinterpret_cast<const float4*>(a.cos + pos * half + p1));
+      sb = __ldg(reinterpret_cast<const float4*>(a.sin + pos * half + p1));
+    }
     c[0] = ca.x, c[1] = ca.y, c[2] = ca.z, c[3] = ca.w, c[4] = cb.x, c[5] = cb.y, c[6] = cb.z, c[7] = cb.w;
     sn[0] = sa.x, sn[1] = sa.y, sn[2] = sa.z, sn[3] = sa.w, sn[4] = sb.x, sn[5] = sb.y, sn[6] = sb.z, sn[7] = sb.w;
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) c[i] = 1.0f, sn[i] = 0.0f;
   }
 #pragma unroll
   for (int s = 0; s < kRotarySteps; ++s) {
@@ -116,17 +135,21 @@ __global__ void __launch_bounds__(kRotaryWarps * 32) rotary_kernel(const RotaryD
     if (hd >= heads) continue;
     const bool is_q = hd < a.HQ, is_k = !is_q && hd < a.HQ + a.HK;
     uint32_t w0[4] = {v0[s].x, v0[s].y, v0[s].z, v0[s].w}, w1[4] = {v1[s].x, v1[s].y, v1[s].z, v1[s].w};
-    if (turned && (is_q || is_k)) {
+    if (is_q || is_k) {
       if (a.interleaved) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           float x, y;
-          rot_unpack<F16>(w0[i], x, y);
-          w0[i] = rot_pack<F16>(fmaf(x, c[i], -(y * sn[i])), fmaf(y, c[i], x * sn[i]));
-          rot_unpack<F16>(w1[i], x, y);
-          w1[i] = rot_pack<F16>(fmaf(x, c[4 + i], -(y * sn[4 + i])), fmaf(y, c[4 + i], x * sn[4 + i]));
+          if (t0) {
+            rot_unpack<F16>(w0[i], x, y);
+            w0[i] = rot_pack<F16>(fmaf(x, c[i], -(y * sn[i])), fmaf(y, c[i], x * sn[i]));
+          }
+          if (t1) {
+            rot_unpack<F16>(w1[i], x, y);
+            w1[i] = rot_pack<F16>(fmaf(x, c[4 + i], -(y * sn[4 + i])), fmaf(y, c[4 + i], x * sn[4 + i]));
+          }
         }
-      } else {
+      } else if (t0) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           float x0, x1, y0, y1;
@@ -151,8 +174,8 @@ __global__ void __launch_bounds__(kRotaryWarps * 32) rotary_kernel(const RotaryD
     } else {
       dst = a.v_out + pg * a.vp_s0 + (hd - a.HQ - a.HK) * a.vp_sh + in_page * a.vp_ss;
     }
-    *reinterpret_cast<uint4*>(dst + c0) = make_uint4(w0[0], w0[1], w0[2], w0[3]);
-    *reinterpret_cast<uint4*>(dst + c1) = make_uint4(w1[0], w1[1], w1[2], w1[3]);
+    __stcs(reinterpret_cast<uint4*>(dst + c0), make_uint4(w0[0], w0[1], w0[2], w0[3]));
+    __stcs(reinterpret_cast<uint4*>(dst + c1), make_uint4(w1[0], w1[1], w1[2], w1[3]));
   }
   pdl_trigger();
 }
