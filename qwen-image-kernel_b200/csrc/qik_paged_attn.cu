@@ -46,11 +46,11 @@ struct PagedDev {
   const int32_t *table, *lens, *starts;
   float* ws_o;        // partial outputs
   float2* ws_ml;      // their (maximum, sum) per row
-  int4* ws_desc;      // split kernel: each CTA's open unit
+  int4* ws_desc;      // each CTA's open unit
   int* status;
   int64_t q_st, q_sh, o_st, o_sh, table_st;
   int B, T, HK, G, W, pages, page_log2, max_new;
-  int window, sinks, splits, min_share;
+  int window, sinks, min_share;
   float scale_log2;
   bool causal, unit_mode;
   int lo_rows, hi_rows;  // rows (new tokens x group) of the sequences this launch takes
@@ -672,7 +672,6 @@ constexpr int kTileM = 128;                    // rows of a query tile (one TMEM
 constexpr int kTileRows = 2 * kTileM;          // rows of a CTA
 constexpr int kTileSoftmaxWarps = 8;           // per query tile: two threads a row
 constexpr int kTileThreads = 128 + 64 * kTileSoftmaxWarps;
-constexpr int kTileLoadWarps = kTileThreads / 32 - 2;  // warps that load q
 constexpr float kTileRescale = 8.0f;           // O is rescaled when a maximum grows by > 2^8
 constexpr int kTilePolyFrom = 23;              // pairs of a half row from here on take 2^x on the FMA pipe
 
@@ -691,62 +690,169 @@ struct TileShape {
   static constexpr int kStages = 2;
   static constexpr int kV0 = kK0 + kStages * kOperand;
   static constexpr int kBar = kV0 + kStages * kOperand;
-  static constexpr int kBytes = kBar + 256 + 1024;
+  static constexpr int kSeg = kBar + 512;                  // segment ring
+  static constexpr int kBytes = kSeg + 4 * 80 + 1024;
   static_assert(kBytes <= 232448, "shared memory above the 227 KB per-CTA limit");
 };
 
-// Which sequence and which 256-row block of it a CTA has: blocks are counted over the
-// sequences that this launch takes.  All threads; `slot` in shared memory.
-__device__ __forceinline__ bool find_block(const PagedDev& a, int block, int* slot, int warps) {
-  // slot[0..1]: sequence, row block; slot[2 ..]: warp sums
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  if (threadIdx.x == 0) slot[0] = -1;
-  int base = 0;
-  for (int i0 = 0; i0 < a.B; i0 += blockDim.x) {
-    const int i = i0 + threadIdx.x;
-    int mine = 0;
-    if (i < a.B) {
-      const int rows = seq_of(a, i).n * a.G;
-      if (rows > a.lo_rows && rows <= a.hi_rows) mine = (rows + kTileRows - 1) / kTileRows;
+// A unit of this kernel is a (sequence, key head, 256-row block); its work is its key tiles.
+struct Block {
+  Seq s;
+  Tiles t;
+  int i, h, rb, blocks;  // sequence, key head, row block, row blocks of the sequence
+  int at, nt;            // tile within the unit, the unit's tiles
+  int left;              // tiles left in the CTA's range
+};
+__device__ __forceinline__ int row_blocks(const PagedDev& a, const Seq& s) {
+  const int rows = s.n * a.G;
+  return rows > a.lo_rows ? (rows + kTileRows - 1) / kTileRows : 0;
+}
+__device__ __forceinline__ Tiles block_tiles(const PagedDev& a, const Seq& s, int rb) {
+  const int row0 = rb * kTileRows, rows = min(s.n * a.G - row0, kTileRows);
+  return tiles_of<kTileN>(a, s, row0 / a.G, (row0 + rows - 1) / a.G + 1);
+}
+// (a unit whose rows see no key still has one tile, so that its rows are written as zeros)
+__device__ __forceinline__ int block_work(const PagedDev& a, const Seq& s, int rb) {
+  const Tiles t = block_tiles(a, s, rb);
+  return max(1, t.sink + t.main);
+}
+// Tiles of all row blocks of the sequence of one key head.  Whole warp: lanes with few
+// blocks add theirs up alone, the others' blocks are shared out over the warp.
+__device__ __forceinline__ int sequence_work(const PagedDev& a, const Seq& s, int blocks) {
+  int sum = 0;
+  if (blocks <= 4)
+    for (int rb = 0; rb < blocks; ++rb) sum += block_work(a, s, rb);
+  for (uint32_t big = __ballot_sync(0xffffffffu, blocks > 4); big; big &= big - 1) {
+    const int l = __ffs(big) - 1;
+    Seq o;
+    o.q0 = 0;
+    o.n = __shfl_sync(0xffffffffu, s.n, l);
+    o.kv = __shfl_sync(0xffffffffu, s.kv, l);
+    const int n = __shfl_sync(0xffffffffu, blocks, l);
+    int part = 0;
+    for (int rb = threadIdx.x & 31; rb < n; rb += 32) part += block_work(a, o, rb);
+    part = __reduce_add_sync(0xffffffffu, part);
+    if (static_cast<int>(threadIdx.x & 31) == l) sum = part;
+  }
+  return sum;
+}
+__device__ __forceinline__ void open_block(const PagedDev& a, Block& b) {
+  b.t = block_tiles(a, b.s, b.rb);
+  b.nt = max(1, b.t.sink + b.t.main);
+}
+__device__ __forceinline__ bool next_block(const PagedDev& a, Block& b, int taken) {
+  b.left -= taken;
+  if (b.left <= 0) return false;
+  b.at = 0;
+  if (++b.rb == b.blocks) {
+    b.rb = 0;
+    if (++b.h == a.HK) {
+      b.h = 0;
+      do {
+        if (++b.i >= a.B) return false;
+        b.s = seq_of(a, b.i);
+        b.blocks = row_blocks(a, b.s);
+      } while (b.blocks == 0);
     }
-    int incl = mine;
+  }
+  open_block(a, b);
+  return true;
+}
+// The CTA's range of tiles: an equal share of all of them, counted sequence by sequence, head
+// by head, row block by row block.  All threads; `slot`: 32 ints of shared memory.
+__device__ __forceinline__ bool open_range(const PagedDev& a, Block& b, int& share, int* slot) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  Seq s;
+  int blocks, mine = 0, sum = 0;
+  auto look = [&](int i) {
+    s = seq_of(a, min(i, a.B - 1));
+    blocks = i < a.B ? row_blocks(a, s) : 0;
+    mine = sequence_work(a, s, blocks) * a.HK;
+  };
+  auto scan_block = [&](int v, int& total) {  // what the threads before this one hold, and all
+    int incl = v;
+#pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int up = __shfl_up_sync(0xffffffffu, incl, o);
       if (lane >= o) incl += up;
     }
     __syncthreads();
-    if (lane == 31) slot[2 + warp] = incl;
+    if (lane == 31) slot[4 + warp] = incl;
     __syncthreads();
-    for (int k = 0; k < warp; ++k) incl += slot[2 + k];
-    const int excl = base + incl - mine;
-    if (mine > 0 && excl <= block && block < excl + mine) {
-      slot[0] = i;
-      slot[1] = block - excl;
+    total = 0;
+    for (int k = 0; k < warps; ++k) {
+      if (k == warp) incl += total;
+      total += slot[4 + k];
     }
-    for (int k = 0; k < warps; ++k) base += slot[2 + k];
-    if (base > block) break;
+    return incl - v;
+  };
+  for (int i0 = 0; i0 < a.B; i0 += blockDim.x) {
+    look(i0 + threadIdx.x);
+    sum += mine;
+  }
+  int total, excl = scan_block(sum, total);
+  share = max(a.min_share, static_cast<int>((static_cast<uint32_t>(total) + gridDim.x - 1) / gridDim.x));
+  const long long begin = static_cast<long long>(share) * blockIdx.x;
+  if (begin >= total) return false;
+  const int want = static_cast<int>(begin);
+  b.left = min(share, total - want);
+  int base = 0;
+  for (int i0 = 0; i0 < a.B; i0 += blockDim.x) {
+    if (a.B > static_cast<int>(blockDim.x)) {
+      look(i0 + threadIdx.x);
+      excl = base + scan_block(mine, total);
+      base += total;
+    }
+    if (mine > 0 && excl <= want && want < excl + mine) {
+      slot[0] = i0 + threadIdx.x;
+      slot[1] = (want - excl) / (mine / a.HK);
+      slot[2] = (want - excl) % (mine / a.HK);
+    }
+    if (base > want) break;
   }
   __syncthreads();
-  return slot[0] >= 0;
+  b.i = slot[0];
+  b.h = slot[1];
+  b.s = seq_of(a, b.i);
+  b.blocks = row_blocks(a, b.s);
+  int rest = slot[2];
+  for (int rb0 = 0;; rb0 += 32) {  // the row block that holds tile `rest` (every warp for itself)
+    const int rb = rb0 + lane;
+    const int work = rb < b.blocks ? block_work(a, b.s, rb) : 0;
+    int incl = work;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += up;
+    }
+    const uint32_t past = __ballot_sync(0xffffffffu, incl > rest);
+    if (past) {
+      const int l = __ffs(past) - 1;
+      b.rb = rb0 + l;
+      b.at = rest - __shfl_sync(0xffffffffu, incl - work, l);
+      break;
+    }
+    rest -= __shfl_sync(0xffffffffu, incl, 31);
+    if (rb0 + 32 >= b.blocks) {  // (not reached: `rest` lies in the sequence)
+      b.rb = b.blocks - 1;
+      b.at = 0;
+      break;
+    }
+  }
+  open_block(a, b);
+  return true;
 }
 
-// TMEM accesses of half a row of D columns by each of a row's two threads.
+// 32 of the D / 2 columns of O that each of a row's two threads has.
 template <int D>
-__device__ __forceinline__ void tmem_ld_half(uint32_t addr, uint32_t (&r)[D / 2]) {
-  if constexpr (D == 128) tmem_ld_2x64(addr, r);
+__device__ __forceinline__ void tmem_ld_cols(uint32_t addr, uint32_t (&r)[32]) {
+  if constexpr (D == 128) tmem_ld_2x32(addr, r);
   else tmem_ld_2x32_at32(addr, r);
 }
 template <int D>
-__device__ __forceinline__ void tmem_st_half(uint32_t addr, const uint32_t (&r)[D / 2]) {
-  if constexpr (D == 128) {
-    uint32_t lo[32], hi[32];
-#pragma unroll
-    for (int i = 0; i < 32; ++i) lo[i] = r[i], hi[i] = r[32 + i];
-    tmem_st_2x32(addr, lo);
-    tmem_st_2x32(addr + 32, hi);
-  } else {
-    tmem_st_2x32_at32(addr, r);
-  }
+__device__ __forceinline__ void tmem_st_cols(uint32_t addr, const uint32_t (&r)[32]) {
+  if constexpr (D == 128) tmem_st_2x32(addr, r);
+  else tmem_st_2x32_at32(addr, r);
 }
 
 // P half row: the thread's 64 scores, p = 2^(s * scale - m) in pairs, packed over its own
@@ -777,6 +883,28 @@ __device__ __forceinline__ float tile_softmax(const float (&sv)[64], float scale
   return f2_sum(acc[0]) + f2_sum(acc[1]);
 }
 
+// What the warps know of a segment, in a ring in shared memory: kept there so that the softmax
+// threads, which hold half a score row each, have their registers for that.
+struct Segment {
+  int valid, i, q0, h, row0, rows;  // sequence, its first row of q, key head, packed rows of the block
+  int n, n0, n1;                    // key tiles; of them, those that query tiles 0 and 1 need
+  int kv0, sink_end, main0;         // first key; where the sink tiles end and the others begin
+  int lmin, lmax, offset, kv;       // keys that some row sees; place of new token 0; tokens
+  int begins, ends, pieces, pad;    // first / last segment of its unit; CTAs that follow with more of it
+};
+static_assert(sizeof(Segment) == 80, "segment ring");
+constexpr int kSegRing = 4;
+
+// One CTA per SM walks its range of the units' key tiles (open_range) segment by segment; a
+// segment is a run of one unit's tiles.  All rings and barriers run on from segment to segment:
+// the producer is ahead with the next segment's K and V while this one's last rows are stored.
+//   warp 0      K and V tiles by TMA into 2-stage rings, V one tile behind K;
+//   warp 1      MMA issuer (one thread): per tile t and query tile g, O_g += P_g(t) V_t, then
+//               S_g(t + 1) = Q_g K_{t+1}^T (qik_attn.cu has the ordering argument);
+//   warps 2-3   q rows of the next segment into shared memory once the last S is done; warp 2
+//               also zeroes V rows that no row of the block sees, warp 3 writes the segments;
+//   warps 4-19  softmax, eight warps per query tile, two threads a row.
+// Query tile 0 ends earlier than tile 1 under a causal mask: its count of tiles is its own.
 template <int D, bool F16>
 __global__ void __launch_bounds__(kTileThreads, 1)
     paged_tile_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
@@ -787,26 +915,28 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Sh::kBar);
   uint64_t* q_full = bars + 0;
-  uint64_t* k_full = bars + 1;    // [2]
-  uint64_t* k_empty = bars + 3;   // [2]
-  uint64_t* v_full = bars + 5;    // [2] V ready for the product
-  uint64_t* v_raw = bars + 7;     // [2] V landed, rows still to be zeroed
-  uint64_t* v_empty = bars + 9;   // [2]
-  uint64_t* s_full = bars + 11;   // [tile]
-  uint64_t* p_full = bars + 13;   // [tile]
-  uint64_t* o_full = bars + 15;   // [tile]
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 17);
+  uint64_t* q_empty = bars + 1;
+  uint64_t* k_full = bars + 2;    // [2]
+  uint64_t* k_empty = bars + 4;   // [2]
+  uint64_t* v_full = bars + 6;    // [2] V ready for the product
+  uint64_t* v_raw = bars + 8;     // [2] V landed, rows still to be zeroed
+  uint64_t* v_empty = bars + 10;  // [2]
+  uint64_t* s_full = bars + 12;   // [tile]
+  uint64_t* p_full = bars + 14;   // [tile]
+  uint64_t* o_full = bars + 16;   // [tile] the segment's last product is done
+  uint64_t* o_empty = bars + 18;  // [tile] O has been read
+  uint64_t* seg_full = bars + 20;   // [kSegRing]
+  uint64_t* seg_empty = bars + 24;  // [kSegRing]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 28);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  int* slot = reinterpret_cast<int*>(tmem_slot + 2);  // find_block: 2 + 20 words
+  int* slot = reinterpret_cast<int*>(tmem_slot + 2);  // open_range: 4 + 20 words
+  volatile Segment* ring = reinterpret_cast<volatile Segment*>(smem + Sh::kSeg);
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
-  // heaviest first: under causal masks the last blocks of a sequence see the most keys
-  const int block = static_cast<int>(gridDim.y - 1 - blockIdx.y);
-  const int h = blockIdx.x;
-
   if (threadIdx.x == 0) {
-    mbar_init(q_full, kTileLoadWarps);
+    mbar_init(q_full, 2);
+    mbar_init(q_empty, 1);
     for (int s = 0; s < 2; ++s) {
       mbar_init(&k_full[s], 1);
       mbar_init(&k_empty[s], 1);
@@ -816,19 +946,25 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       mbar_init(&s_full[s], 1);
       mbar_init(&p_full[s], kTileSoftmaxWarps);
       mbar_init(&o_full[s], 1);
+      mbar_init(&o_empty[s], kTileSoftmaxWarps);
+    }
+    for (int s = 0; s < kSegRing; ++s) {
+      mbar_init(&seg_full[s], 1);
+      mbar_init(&seg_empty[s], 3 + 2 * kTileSoftmaxWarps);  // warps 0, 1 and 2, softmax
     }
     *abort_flag = 0;
     fence_mbar_init();
   }
   pdl_wait();
-  __syncthreads();
-  if (blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0) report_bad_lengths(a);
-  if (!find_block(a, block, slot, kTileThreads / 32)) {
+  if (blockIdx.x == 0) report_bad_lengths(a);
+  Block b;
+  int share;
+  const bool any = open_range(a, b, share, slot);
+  if (threadIdx.x == 0) a.ws_desc[2 * blockIdx.x] = make_int4(-1, 0, 0, 0);
+  if (!any) {
     pdl_trigger();
     return;
   }
-  const int seq = slot[0];
-  const int row0 = slot[1] * kTileRows;  // first packed row of this CTA
   if (warp == 1) {
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
@@ -837,267 +973,379 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  const Seq s = seq_of(a, seq);
-  const int rows = min(s.n * a.G - row0, kTileRows);
-  const int n_q = rows > kTileM ? 2 : 1;  // query tiles with rows
-  const Tiles tl = tiles_of<kTileN>(a, s, row0 / a.G, (row0 + rows - 1) / a.G + 1);
-  const int all_tiles = tl.sink + tl.main;
-  const int first = static_cast<int>(static_cast<int64_t>(all_tiles) * blockIdx.z / a.splits);
-  const int n_tiles = static_cast<int>(static_cast<int64_t>(all_tiles) * (blockIdx.z + 1) / a.splits) - first;
-  auto kv_of = [&](int t) { return tile_at(tl, first + t) * kTileN; };
-  // V rows of the tile that no row of this CTA sees
-  auto edge = [&](int kv0) { return kv0 + kTileN - 1 > tl.lmax || (kv0 < tl.lmin && kv0 + kTileN - 1 >= a.sinks); };
 
   uint8_t* sQ = smem;
   auto k_ptr = [&](int st) { return smem + Sh::kK0 + st * Sh::kOperand; };
   auto v_ptr = [&](int st) { return smem + Sh::kV0 + st * Sh::kOperand; };
-
-  if (warp >= 2 && n_tiles > 0) {
-    // q rows into the 128-byte-swizzled tiles; rows behind the last are zeros
-    for (int x = threadIdx.x - 64; x < n_q * kTileM * (D / 8); x += kTileLoadWarps * 32) {
-      const int r = x / (D / 8), ch = x % (D / 8);
-      uint4 v = make_uint4(0u, 0u, 0u, 0u);
-      if (r < rows) {
-        const int pr = row0 + r, j = pr / a.G, hq = h * a.G + pr % a.G;
-        v = __ldg(reinterpret_cast<const uint4*>(a.q + static_cast<int64_t>(s.q0 + j) * a.q_st +
-                                                 static_cast<int64_t>(hq) * a.q_sh) + ch);
-      }
-      const int rr = r & 127;
-      *reinterpret_cast<uint4*>(sQ + (r >> 7) * Sh::kOperand + (ch >> 3) * Sh::kHalfBytes + rr * 128 +
-                                (((ch & 7) ^ (rr & 7)) << 4)) = v;
-    }
-    fence_proxy_async_smem();
-    __syncwarp();
-    if (lane == 0) mbar_arrive(q_full);
-  }
+  // segment number n of the CTA, or a segment that is not valid when a wait gave up
+  auto seg_wait = [&](uint32_t n) -> bool {
+    const bool ok = mbar_wait(&seg_full[n & (kSegRing - 1)], (n / kSegRing) & 1, abort_flag, a.status);
+    return ok && ring[n & (kSegRing - 1)].valid;
+  };
+  auto kv_next = [](int kv0, int sink_end, int main0) { return kv0 + kTileN == sink_end ? main0 : kv0 + kTileN; };
+  // V rows of the tile that no row of the block sees
+  auto edge = [&](int kv0, int lmin, int lmax) {
+    return kv0 + kTileN - 1 > lmax || (kv0 < lmin && kv0 + kTileN - 1 >= a.sinks);
+  };
 
   if (warp == 0) {
     // ------------------------------------------------------------ producer
     const int page = 1 << a.page_log2;
     const int box = min(page, kTileN);
     const int pieces = kTileN / box;
-    const int32_t* row = a.table + static_cast<int64_t>(seq) * a.table_st;
-    auto page_of = [&](int t) {
-      if (lane >= pieces || t >= n_tiles) return -1;
-      const int key = kv_of(t) + lane * box;
-      const int p = key >> a.page_log2;
-      if (key >= s.kv || p >= a.W) return -1;
-      const int id = __ldg(row + p);
-      if ((id < 0 || id >= a.pages) && a.status) atomicExch(a.status, QIK_DEV_BAD_INDEX);
-      return id < a.pages ? id : -1;
-    };
-    auto load = [&](const CUtensorMap* tm, uint8_t* dst, int t, int id, uint64_t* bar) {
+    uint32_t n_k = 0;  // tiles issued so far
+    // the previous tile, whose V is still to be loaded
+    int v_id = -1, v_place = 0, v_h = 0;
+    bool v_edge = false, ok = true;
+    auto load = [&](const CUtensorMap* tm, uint8_t* dst, int id, int place, int h, uint64_t* bar) {
       if (lane == 0) mbar_arrive_expect_tx(bar, Sh::kOperand);
       __syncwarp();
       if (lane < pieces) {
-        const int place = (kv_of(t) + lane * box) & (page - 1);
 #pragma unroll
         for (int hd = 0; hd < Sh::kHalves; ++hd)
           tma_load_5d(dst + hd * Sh::kHalfBytes + lane * box * 128, tm, 0, place, hd, h, id, bar);
       }
     };
-    // step u: K of tile u, then V of tile u - 1
-    int next = page_of(0), cur = -1, prev;
-    for (int u = 0; u <= n_tiles && n_tiles > 0; ++u) {
-      prev = cur;
-      cur = next;
-      next = page_of(u + 1);
-      if (u < n_tiles) {
-        const int st = u & 1;
-        if (!__all_sync(0xffffffffu, mbar_wait(&k_empty[st], ((u >> 1) & 1) ^ 1u, abort_flag, a.status))) break;
-        load(&tm_k, k_ptr(st), u, cur, &k_full[st]);
-      }
-      const int t = u - 1;
-      if (t >= 0) {
-        const int st = t & 1;
-        if (!__all_sync(0xffffffffu, mbar_wait(&v_empty[st], ((t >> 1) & 1) ^ 1u, abort_flag, a.status))) break;
-        load(&tm_v, v_ptr(st), t, prev, edge(kv_of(t)) ? &v_raw[st] : &v_full[st]);
+    auto load_v = [&](uint32_t t) {  // V of tile t of the CTA
+      const int st = t & 1;
+      ok = ok && __all_sync(0xffffffffu, mbar_wait(&v_empty[st], ((t >> 1) & 1) ^ 1u, abort_flag, a.status));
+      if (ok) load(&tm_v, v_ptr(st), v_id, v_place, v_h, v_edge ? &v_raw[st] : &v_full[st]);
+    };
+    for (uint32_t seg = 0; ok && __all_sync(0xffffffffu, seg_wait(seg)); ++seg) {
+      volatile Segment* sg = ring + (seg & (kSegRing - 1));
+      const int n = sg->n, h = sg->h, kv = sg->kv, lmin = sg->lmin, lmax = sg->lmax, sink_end = sg->sink_end, main0 = sg->main0;
+      int kv0 = sg->kv0;
+      const int32_t* row = a.table + static_cast<int64_t>(sg->i) * a.table_st;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&seg_empty[seg & (kSegRing - 1)]);
+      auto page_of = [&](int first) {
+        if (lane >= pieces) return -1;
+        const int key = first + lane * box;
+        const int p = key >> a.page_log2;
+        if (key >= kv || p >= a.W) return -1;
+        const int id = __ldg(row + p);
+        if ((id < 0 || id >= a.pages) && a.status) atomicExch(a.status, QIK_DEV_BAD_INDEX);
+        return id < a.pages ? id : -1;
+      };
+      int next = n > 0 ? page_of(kv0) : -1;
+      for (int t = 0; t < n && ok; ++t, ++n_k) {
+        const int id = next, kv1 = kv_next(kv0, sink_end, main0);
+        next = t + 1 < n ? page_of(kv1) : -1;
+        const int st = n_k & 1, place = (kv0 + lane * box) & (page - 1);
+        ok = __all_sync(0xffffffffu, mbar_wait(&k_empty[st], ((n_k >> 1) & 1) ^ 1u, abort_flag, a.status));
+        if (!ok) break;
+        load(&tm_k, k_ptr(st), id, place, h, &k_full[st]);
+        if (n_k > 0) load_v(n_k - 1);
+        v_id = id, v_place = place, v_h = h, v_edge = edge(kv0, lmin, lmax);
+        kv0 = kv1;
       }
     }
+    if (n_k > 0 && ok) load_v(n_k - 1);
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer
-    if (lane == 0 && n_tiles > 0) {
+    if (lane == 0) {
       constexpr uint32_t fmt = F16 ? 0 : 1;
       constexpr uint32_t idesc_s = idesc_f32acc(fmt, fmt, 0, 0, kTileM, kTileN);
       constexpr uint32_t idesc_o = idesc_f32acc(fmt, fmt, 0, 1, kTileM, D);
-      bool ok = mbar_wait(q_full, 0, abort_flag, a.status);
-      tc_fence_after();
       const uint64_t q_desc = sdesc_sw128(smem_u32(sQ), 16, 1024);
       const uint64_t k_desc = sdesc_sw128(smem_u32(k_ptr(0)), 16, 1024);
       const uint64_t v_desc = sdesc_sw128(smem_u32(v_ptr(0)), Sh::kHalfBytes, 1024);
       constexpr uint64_t kOp16 = Sh::kOperand >> 4;
-      auto issue_s = [&](int g, int t) {
-        const uint64_t qd = q_desc + g * kOp16, kd = k_desc + static_cast<uint64_t>(t & 1) * kOp16;
+      uint32_t base = 0, q_n = 0, p_n[2] = {0u, 0u}, o_n[2] = {0u, 0u};  // tiles, q loads, P and O so far
+      bool ok = true;
+      auto wait = [&](uint64_t* bar, uint32_t parity) { ok = ok && mbar_wait(bar, parity & 1u, abort_flag, a.status); };
+      auto issue_s = [&](int g, uint32_t k) {  // k: the CTA's tile
+        const uint64_t qd = q_desc + g * kOp16, kd = k_desc + static_cast<uint64_t>(k & 1) * kOp16;
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-          const uint32_t off16 = ((k >> 2) * Sh::kHalfBytes + (k & 3) * 32) >> 4;
-          umma_f16_ss(tmem + 128u * g, qd + off16, kd + off16, idesc_s, k > 0 ? 1u : 0u);
+        for (int i = 0; i < D / 16; ++i) {
+          const uint32_t off16 = ((i >> 2) * Sh::kHalfBytes + (i & 3) * 32) >> 4;
+          umma_f16_ss(tmem + 128u * g, qd + off16, kd + off16, idesc_s, i > 0 ? 1u : 0u);
         }
         umma_commit(&s_full[g]);
       };
-      auto wait_k = [&](int t) -> bool {
-        if (!mbar_wait(&k_full[t & 1], (t >> 1) & 1, abort_flag, a.status)) return false;
-        tc_fence_after();
-        return true;
-      };
-      auto issue_pv = [&](int g, int t) -> bool {
-        const int st = t & 1;
-        if (!mbar_wait(&p_full[g], t & 1, abort_flag, a.status)) return false;
-        if (g == 0 && !mbar_wait(&v_full[st], (t >> 1) & 1, abort_flag, a.status)) return false;
-        tc_fence_after();
-        const uint64_t vd = v_desc + static_cast<uint64_t>(st) * kOp16;
+      auto issue_pv = [&](int g, uint32_t k, bool first) {
+        const uint64_t vd = v_desc + static_cast<uint64_t>(k & 1) * kOp16;
 #pragma unroll
-        for (int k = 0; k < kTileN / 16; ++k) {
-          const uint32_t p_col = 128u * g + k * 8 + (k >= kTileN / 32 ? 32u : 0u);
-          umma_f16_ts(tmem + 256u + 128u * g, tmem + p_col, vd + k * 128u, idesc_o, (t > 0 || k > 0) ? 1u : 0u);
+        for (int i = 0; i < kTileN / 16; ++i) {
+          const uint32_t p_col = 128u * g + i * 8 + (i >= kTileN / 32 ? 32u : 0u);
+          umma_f16_ts(tmem + 256u + 128u * g, tmem + p_col, vd + i * 128u, idesc_o, !first || i > 0 ? 1u : 0u);
         }
-        if (t == n_tiles - 1) umma_commit(&o_full[g]);
-        if (g == n_q - 1) umma_commit(&v_empty[st]);
-        return true;
       };
-      if (ok && wait_k(0)) {
-        for (int g = 0; g < n_q; ++g) issue_s(g, 0);
-        umma_commit(&k_empty[0]);
-        for (int t = 0; t < n_tiles && ok; ++t) {
-          const bool more = t + 1 < n_tiles;
-          for (int g = 0; g < n_q && ok; ++g) {
-            ok = issue_pv(g, t);
-            if (ok && more) {
-              if (g == 0) ok = wait_k(t + 1);
-              if (ok) issue_s(g, t + 1);
+      for (uint32_t seg = 0; ok && seg_wait(seg); ++seg) {
+        volatile Segment* sg = ring + (seg & (kSegRing - 1));
+        const int n = sg->n, n0 = sg->n0, n1 = sg->n1, most = max(n0, n1);
+        mbar_arrive(&seg_empty[seg & (kSegRing - 1)]);
+        if (n == 0) continue;
+        wait(q_full, q_n++);
+        wait(&k_full[base & 1], base >> 1);
+        tc_fence_after();
+        if (ok) {
+          if (n0 > 0) issue_s(0, base);
+          if (n1 > 0) issue_s(1, base);
+          umma_commit(&k_empty[base & 1]);
+          if (most <= 1) umma_commit(q_empty);
+        }
+        for (int t = 0; t < n && ok; ++t) {
+          const uint32_t k = base + t;
+#pragma unroll
+          for (int g = 0; g < 2; ++g) {  // (unrolled: p_n and o_n stay in registers)
+            const int mine = g == 0 ? n0 : n1;
+            if (ok && t < mine) {
+              wait(&p_full[g], p_n[g]++);
+              if (g == 0 || n0 <= t) wait(&v_full[k & 1], k >> 1);
+              if (t == 0 && o_n[g] > 0) wait(&o_empty[g], o_n[g] - 1);
+              if (ok) {
+                tc_fence_after();
+                issue_pv(g, k, t == 0);
+                if (t == mine - 1) {
+                  umma_commit(&o_full[g]);
+                  ++o_n[g];
+                }
+              }
+            }
+            if (g == 1 && ok) umma_commit(&v_empty[k & 1]);
+            if (ok && t + 1 < mine) {
+              if (g == 0 || n0 <= t + 1) {
+                wait(&k_full[(k + 1) & 1], (k + 1) >> 1);
+                tc_fence_after();
+              }
+              if (ok) issue_s(g, k + 1);
             }
           }
-          if (ok && more) umma_commit(&k_empty[(t + 1) & 1]);
+          if (!ok) break;
+          if (t + 1 < n) umma_commit(&k_empty[(k + 1) & 1]);
+          if (most > 1 && t + 2 == most) umma_commit(q_empty);
         }
+        base += n;
       }
     }
-  } else if (warp == 2) {
-    // ------------------------------------------------------------ V rows nobody sees
-    uint32_t seen[2] = {0u, 0u};
-    for (int t = 0; t < n_tiles; ++t) {
-      const int kv0 = kv_of(t), st = t & 1;
-      if (!edge(kv0)) continue;
-      if (!__all_sync(0xffffffffu, mbar_wait(&v_raw[st], seen[st]++ & 1u, abort_flag, a.status))) break;
-      for (int key = lane >> 3; key < kTileN; key += 4) {
-        const int kv = kv0 + key;
-        if (kv > tl.lmax || (kv < tl.lmin && kv >= a.sinks)) {
-#pragma unroll
-          for (int hd = 0; hd < Sh::kHalves; ++hd)
-            *reinterpret_cast<uint4*>(v_ptr(st) + hd * Sh::kHalfBytes + key * 128 + ((lane & 7) << 4)) =
-                make_uint4(0u, 0u, 0u, 0u);
+  } else if (warp < 4) {
+    // ------------------------------------------------------------ q rows; V rows nobody sees
+    uint32_t base = 0, q_n = 0, seen[2] = {0u, 0u};
+    bool ok = true, more = true;
+    for (uint32_t seg = 0; ok; ++seg) {
+      volatile Segment* sg = ring + (seg & (kSegRing - 1));
+      if (warp == 3) {  // writes the segment (or the end)
+        if (seg >= kSegRing)
+          ok = __all_sync(0xffffffffu, mbar_wait(&seg_empty[seg & (kSegRing - 1)], (seg / kSegRing - 1) & 1, abort_flag, a.status));
+        if (!ok) break;
+        if (lane == 0) {
+          sg->valid = more;
+          if (more) {
+            const int rows = min(b.s.n * a.G - b.rb * kTileRows, kTileRows), row0 = b.rb * kTileRows;
+            const int taken = min(b.nt - b.at, b.left), n = b.t.main == 0 ? 0 : taken;
+            const int last = last_key(a, b.s, (row0 + min(rows, kTileM) - 1) / a.G);
+            sg->i = b.i, sg->q0 = b.s.q0, sg->h = b.h, sg->row0 = row0, sg->rows = rows;
+            sg->n = n;
+            sg->n0 = last < 0 ? 0 : max(0, min(n, b.t.sink + last / kTileN - b.t.t0 + 1 - b.at));
+            sg->n1 = rows > kTileM ? n : 0;
+            sg->kv0 = tile_at(b.t, b.at) * kTileN;
+            sg->sink_end = b.t.sink > 0 ? b.t.sink * kTileN : -1;
+            sg->main0 = b.t.t0 * kTileN;
+            sg->lmin = b.t.lmin, sg->lmax = b.t.lmax, sg->kv = b.s.kv;
+            sg->offset = b.s.kv - b.s.n;
+            sg->begins = b.at == 0, sg->ends = b.at + taken == b.nt;
+            sg->pieces = (b.nt - b.at - taken + share - 1) / share;
+          }
+          mbar_arrive(&seg_full[seg & (kSegRing - 1)]);
         }
-      }
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&v_full[st]);
-    }
-  } else if (warp >= 4) {
-    // ------------------------------------------------------------ softmax (tile g)
-    const int sw = warp - 4;
-    const int g = sw >> 3;
-    const int quarter = sw & 3;      // TMEM lane quarter (warp % 4)
-    const int sub = (sw >> 2) & 1;   // its lower or upper 16 lanes
-    const int hc = lane >> 4;        // column half of the row
-    const int r = g * kTileM + quarter * 32 + sub * 16 + (lane & 15);
-    const uint32_t lane_base = static_cast<uint32_t>(quarter * 32 + sub * 16) << 16;
-    const uint32_t tS = tmem + lane_base + 128u * g;
-    const uint32_t tO = tmem + lane_base + 256u + 128u * g;
-    const int pr = row0 + min(r, rows - 1);  // rows behind the last follow it and are not stored
-    const int j = pr / a.G, hq = h * a.G + pr % a.G;
-    const int my_last = last_key(a, s, j), my_first = first_key(a, my_last);
-    float m_run = -INFINITY, l_run = 0.0f;
-    bool ok = true;
-    const int work = g < n_q ? n_tiles : 0;
-    for (int t = 0; t < work; ++t) {
-      if (!__all_sync(0xffffffffu, mbar_wait(&s_full[g], t & 1, abort_flag, a.status))) {
-        ok = false;
-        break;
-      }
-      tc_fence_after();
-      const int kv0 = kv_of(t);
-      float sv[64];
-      {
-        uint32_t rr[64];
-        tmem_ld_2x64(tS, rr);
-#pragma unroll
-        for (int i = 0; i < 64; ++i) sv[i] = __uint_as_float(rr[i]);
-      }
-      const bool whole = __all_sync(0xffffffffu, kv0 + kTileN - 1 <= my_last &&
-                                                     (kv0 >= my_first || kv0 + kTileN - 1 < a.sinks));
-      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-      if (whole) {
-#pragma unroll
-        for (int c = 0; c < 64; c += 8) {
-          mx[0] = fmax3_nan(mx[0], sv[c], sv[c + 1]);
-          mx[1] = fmax3_nan(mx[1], sv[c + 2], sv[c + 3]);
-          mx[2] = fmax3_nan(mx[2], sv[c + 4], sv[c + 5]);
-          mx[3] = fmax3_nan(mx[3], sv[c + 6], sv[c + 7]);
-        }
+        __syncwarp();
+        if (!more) break;
+        more = next_block(a, b, min(b.nt - b.at, b.left));
       } else {
-        const int col0 = kv0 + 64 * hc;
-        const int last = my_last - col0, low = my_first - col0, sink = a.sinks - col0;
+        ok = __all_sync(0xffffffffu, seg_wait(seg));
+        if (!ok) break;
+      }
+      const int n = sg->n, rows = sg->rows, row0 = sg->row0, q0 = sg->q0, h = sg->h, lmin = sg->lmin, lmax = sg->lmax,
+                sink_end = sg->sink_end, main0 = sg->main0;
+      int kv0 = sg->kv0;
+      __syncwarp();
+      if (warp == 2 && lane == 0) mbar_arrive(&seg_empty[seg & (kSegRing - 1)]);
+      if (n == 0) continue;
+      if (q_n > 0) ok = __all_sync(0xffffffffu, mbar_wait(q_empty, (q_n - 1) & 1, abort_flag, a.status));
+      if (!ok) break;
+      ++q_n;
+      {  // a thread has one 16-byte chunk of every kStep-th row
+        constexpr int kChunks = D / 8, kStep = 64 / kChunks;
+        const int n_rows = rows > kTileM ? kTileRows : kTileM;
+        const int x = threadIdx.x - 64, ch = x % kChunks;
+        int r = x / kChunks;
+        const int pr = row0 + r, j = pr / a.G;
+        int gg = pr % a.G;
+        const int dj = kStep / a.G, dg = kStep % a.G;
+        const uint16_t* src = a.q + static_cast<int64_t>(q0 + j) * a.q_st + static_cast<int64_t>(h * a.G + gg) * a.q_sh + ch * 8;
+        const int64_t step = dj * a.q_st + dg * a.q_sh, wrap = a.q_st - a.G * a.q_sh;
+        const uint32_t dst = smem_u32(sQ) + (ch >> 3) * Sh::kHalfBytes;
+        for (; r < n_rows; r += kStep) {
+          const int rr = r & 127;
+          cp_async16(dst + (r >> 7) * Sh::kOperand + rr * 128 + (((ch & 7) ^ (rr & 7)) << 4), r < rows ? src : a.q, r < rows);
+          src += step;
+          gg += dg;
+          if (gg >= a.G) {
+            gg -= a.G;
+            src += wrap;
+          }
+        }
+        cp_async_wait_all();
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(q_full);
+      }
+      for (int t = 0; t < n && warp == 2; ++t) {
+        const int st = (base + t) & 1;
+        if (edge(kv0, lmin, lmax)) {
+          ok = __all_sync(0xffffffffu, mbar_wait(&v_raw[st], seen[st]++ & 1u, abort_flag, a.status));
+          if (!ok) break;
+          for (int key = lane >> 3; key < kTileN; key += 4) {
+            const int kv = kv0 + key;
+            if (kv > lmax || (kv < lmin && kv >= a.sinks)) {
 #pragma unroll
-        for (int c = 0; c < 64; ++c) {
-          sv[c] = c <= last && (c >= low || c < sink) ? sv[c] : -INFINITY;
-          mx[c & 3] = fmaxf(mx[c & 3], sv[c]);
+              for (int hd = 0; hd < Sh::kHalves; ++hd)
+                *reinterpret_cast<uint4*>(v_ptr(st) + hd * Sh::kHalfBytes + key * 128 + ((lane & 7) << 4)) =
+                    make_uint4(0u, 0u, 0u, 0u);
+            }
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&v_full[st]);
+        }
+        kv0 = kv_next(kv0, sink_end, main0);
+      }
+      base += n;
+    }
+  } else {
+    // ------------------------------------------------------------ softmax (tile g)
+    const int g = (warp - 4) >> 3;
+    const int hc = lane >> 4;  // column half of the row
+    // TMEM lane quarter warp % 4, its lower or upper 16 lanes by (warp / 4) % 2
+    const int lane0 = (warp & 3) * 32 + (((warp - 4) >> 2) & 1) * 16;
+    const int r = g * kTileM + lane0 + (lane & 15);
+    const uint32_t tS = tmem + (static_cast<uint32_t>(lane0) << 16) + 128u * g;
+    const uint32_t tO = tS + 256u;
+    uint32_t s_n = 0, o_n = 0;  // S tiles and segments of this query tile so far
+    bool ok = true;
+    for (uint32_t seg = 0; ok && __all_sync(0xffffffffu, seg_wait(seg)); ++seg) {
+      volatile Segment* sg = ring + (seg & (kSegRing - 1));
+      const int work = g == 0 ? sg->n0 : sg->n1;
+      int my_last, my_first, kv0 = sg->kv0;
+      {
+        const int j = (sg->row0 + min(r, sg->rows - 1)) / a.G;  // rows behind the last follow it, unstored
+        my_last = a.causal ? sg->offset + j : sg->kv - 1;
+        my_first = first_key(a, my_last);
+      }
+      float m_run = -INFINITY, l_run = 0.0f;
+      for (int t = 0; t < work; ++t, ++s_n) {
+        if (!__all_sync(0xffffffffu, mbar_wait(&s_full[g], s_n & 1, abort_flag, a.status))) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        float sv[64];
+        {
+          uint32_t rr[64];
+          tmem_ld_2x64(tS, rr);
+#pragma unroll
+          for (int i = 0; i < 64; ++i) sv[i] = __uint_as_float(rr[i]);
+        }
+        const bool whole = __all_sync(0xffffffffu, kv0 + kTileN - 1 <= my_last &&
+                                                       (kv0 >= my_first || kv0 + kTileN - 1 < a.sinks));
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        if (whole) {
+#pragma unroll
+          for (int c = 0; c < 64; c += 8) {
+            mx[0] = fmax3_nan(mx[0], sv[c], sv[c + 1]);
+            mx[1] = fmax3_nan(mx[1], sv[c + 2], sv[c + 3]);
+            mx[2] = fmax3_nan(mx[2], sv[c + 4], sv[c + 5]);
+            mx[3] = fmax3_nan(mx[3], sv[c + 6], sv[c + 7]);
+          }
+        } else {
+          const int col0 = kv0 + 64 * hc;
+          const int last = my_last - col0, low = my_first - col0, sink = a.sinks - col0;
+#pragma unroll
+          for (int c = 0; c < 64; ++c) {
+            sv[c] = c <= last && (c >= low || c < sink) ? sv[c] : -INFINITY;
+            mx[c & 3] = fmaxf(mx[c & 3], sv[c]);
+          }
+        }
+        // a NaN score reaches the row's sum through its maximum: 2^x on the FMA pipe clamps it
+        float raw_max = fmax3_nan(mx[0], mx[1], mx[2]);
+        raw_max = fmax3_nan(raw_max, mx[3], __shfl_xor_sync(0xffffffffu, fmax3_nan(raw_max, mx[3], mx[3]), 16));
+        const float tmax = raw_max * a.scale_log2;
+        float alpha = 1.0f;
+        bool rescale = false;
+        if (tmax > m_run + kTileRescale || (m_run == -INFINITY && tmax > -INFINITY)) {
+          rescale = m_run != -INFINITY;
+          alpha = rescale ? ex2(m_run - tmax) : 0.0f;
+          m_run = tmax;
+        }
+        const float neg_m = m_run == -INFINITY ? 0.0f : -m_run;
+        const float psum = whole ? tile_softmax<true, F16>(sv, a.scale_log2, neg_m, tS)
+                                 : tile_softmax<false, F16>(sv, a.scale_log2, neg_m, tS);
+        l_run = l_run * alpha + (raw_max == raw_max ? psum : raw_max);
+        if (t >= 1 && __any_sync(0xffffffffu, rescale)) {
+          const float f = rescale ? alpha : 1.0f;
+#pragma unroll
+          for (int c = 0; c < D / 64; ++c) {
+            uint32_t rr[32];
+            tmem_ld_cols<D>(tO + c * 32, rr);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) rr[i] = __float_as_uint(__uint_as_float(rr[i]) * f);
+            tmem_st_cols<D>(tO + c * 32, rr);
+          }
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[g]);
+        kv0 = kv_next(kv0, sg->sink_end, sg->main0);
+      }
+      // ---- O / l, or this segment's piece of the unit
+      const float l_row = l_run + __shfl_xor_sync(0xffffffffu, l_run, 16);
+      if (work > 0 && ok) ok = __all_sync(0xffffffffu, mbar_wait(&o_full[g], o_n++ & 1, abort_flag, a.status));
+      if (!ok) break;
+      tc_fence_after();
+      const int rows = sg->rows, pr = sg->row0 + r;
+      const bool whole = sg->begins && sg->ends;
+      const float inv = !whole ? 1.0f : l_row == 0.0f ? 0.0f : 1.0f / l_row;
+      uint16_t* dst = a.out + static_cast<int64_t>(sg->q0 + pr / a.G) * a.o_st +
+                      static_cast<int64_t>(sg->h * a.G + pr % a.G) * a.o_sh + kHalfO * hc;
+      const int64_t at = static_cast<int64_t>(2 * blockIdx.x + (sg->begins ? 1 : 0)) * kTileRows + r;
+#pragma unroll
+      for (int c = 0; c < D / 64; ++c) {
+        uint32_t o[32];
+        if (work > 0) {
+          tmem_ld_cols<D>(tO + c * 32, o);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = 0u;
+        }
+        if (c == D / 64 - 1 && work > 0) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&o_empty[g]);
+        }
+        if (r < rows && whole) {
+#pragma unroll
+          for (int i = 0; i < 32; i += 8) {
+            uint32_t w[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              w[k] = pack16<F16>(__uint_as_float(o[i + 2 * k]) * inv, __uint_as_float(o[i + 2 * k + 1]) * inv);
+            *reinterpret_cast<uint4*>(dst + c * 32 + i) = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+        } else if (r < rows) {
+          uint4* part = reinterpret_cast<uint4*>(a.ws_o + at * D + kHalfO * hc + c * 32);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) part[i] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
         }
       }
-      // a NaN score reaches the row's sum through its maximum: 2^x on the FMA pipe clamps it
-      float raw_max = fmax3_nan(mx[0], mx[1], mx[2]);
-      raw_max = fmax3_nan(raw_max, mx[3], __shfl_xor_sync(0xffffffffu, fmax3_nan(raw_max, mx[3], mx[3]), 16));
-      const float tmax = raw_max * a.scale_log2;
-      float alpha = 1.0f;
-      bool rescale = false;
-      if (tmax > m_run + kTileRescale || (m_run == -INFINITY && tmax > -INFINITY)) {
-        rescale = m_run != -INFINITY;
-        alpha = rescale ? ex2(m_run - tmax) : 0.0f;
-        m_run = tmax;
+      if (r < rows && !whole && hc == 0) a.ws_ml[at] = make_float2(m_run, l_row);
+      if (warp == 4 && lane == 0 && sg->begins && !sg->ends) {
+        a.ws_desc[2 * blockIdx.x] = make_int4(sg->q0, sg->h, sg->pieces, rows);
+        a.ws_desc[2 * blockIdx.x + 1] = make_int4(sg->row0, 0, 0, 0);
       }
-      const float neg_m = m_run == -INFINITY ? 0.0f : -m_run;
-      const float psum = whole ? tile_softmax<true, F16>(sv, a.scale_log2, neg_m, tS)
-                               : tile_softmax<false, F16>(sv, a.scale_log2, neg_m, tS);
-      l_run = l_run * alpha + (raw_max == raw_max ? psum : raw_max);
-      if (t >= 1 && __any_sync(0xffffffffu, rescale)) {
-        const float f = rescale ? alpha : 1.0f;
-        uint32_t rr[kHalfO];
-        tmem_ld_half<D>(tO, rr);
-#pragma unroll
-        for (int i = 0; i < kHalfO; ++i) rr[i] = __float_as_uint(__uint_as_float(rr[i]) * f);
-        tmem_st_half<D>(tO, rr);
-      }
-      tmem_wait_st();
-      tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&p_full[g]);
-    }
-    // ---- O / l, or the piece of this split
-    const float l_row = l_run + __shfl_xor_sync(0xffffffffu, l_run, 16);
-    float o[kHalfO];
-#pragma unroll
-    for (int i = 0; i < kHalfO; ++i) o[i] = 0.0f;
-    const bool ready = ok && work > 0 && mbar_wait(&o_full[g], 0, abort_flag, a.status);
-    if (__all_sync(0xffffffffu, ready)) {
-      tc_fence_after();
-      uint32_t rr[kHalfO];
-      tmem_ld_half<D>(tO, rr);
-#pragma unroll
-      for (int i = 0; i < kHalfO; ++i) o[i] = __uint_as_float(rr[i]);
-    }
-    if (r < rows && a.splits == 1) {
-      const float inv = l_row == 0.0f ? 0.0f : 1.0f / l_row;
-      uint16_t* dst = a.out + static_cast<int64_t>(s.q0 + j) * a.o_st + static_cast<int64_t>(hq) * a.o_sh + kHalfO * hc;
-#pragma unroll
-      for (int c = 0; c < kHalfO; c += 8)
-        *reinterpret_cast<uint4*>(dst + c) =
-            make_uint4(pack16<F16>(o[c] * inv, o[c + 1] * inv), pack16<F16>(o[c + 2] * inv, o[c + 3] * inv),
-                       pack16<F16>(o[c + 4] * inv, o[c + 5] * inv), pack16<F16>(o[c + 6] * inv, o[c + 7] * inv));
-    } else if (r < rows) {
-      const int64_t at = ((static_cast<int64_t>(blockIdx.z) * gridDim.y + block) * a.HK + h) * kTileRows + r;
-      float* dst = a.ws_o + at * D + kHalfO * hc;
-#pragma unroll
-      for (int c = 0; c < kHalfO; c += 4)
-        *reinterpret_cast<float4*>(dst + c) = make_float4(o[c], o[c + 1], o[c + 2], o[c + 3]);
-      if (hc == 0) a.ws_ml[at] = make_float2(m_run, l_row);
+      if (lane == 0) mbar_arrive(&seg_empty[seg & (kSegRing - 1)]);
     }
   }
   tc_fence_before();
@@ -1109,21 +1357,18 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   }
 }
 
-// Joins the splits of a 256-row block in split order.  One warp a row.
+// Joins the pieces of the unit that CTA blockIdx.x of the tile kernel left open: its own piece,
+// then the following CTAs' first pieces.  Eight rows a CTA.
 template <int D, bool F16>
 __global__ void __launch_bounds__(256) paged_tile_join_kernel(const PagedDev a) {
-  __shared__ int slot[2 + 8];
   pdl_wait();
-  const int block = blockIdx.y, h = blockIdx.x;
-  if (!find_block(a, block, slot, 8)) return;
-  const Seq s = seq_of(a, slot[0]);
-  const int row0 = slot[1] * kTileRows, rows = min(s.n * a.G - row0, kTileRows);
-  const int64_t pitch = static_cast<int64_t>(gridDim.y) * a.HK * kTileRows;
-  for (int r = blockIdx.z * 8 + (threadIdx.x >> 5); r < rows; r += 8 * gridDim.z) {
-    const int64_t at = (static_cast<int64_t>(block) * a.HK + h) * kTileRows + r;
-    const int pr = row0 + r;
-    join_row<D, F16>(a, a.splits, [&](int z) { return at + z * pitch; },
-                     a.out + static_cast<int64_t>(s.q0 + pr / a.G) * a.o_st + static_cast<int64_t>(h * a.G + pr % a.G) * a.o_sh);
+  const int4 d = __ldcg(a.ws_desc + 2 * blockIdx.x), e = __ldcg(a.ws_desc + 2 * blockIdx.x + 1);
+  const int r = blockIdx.y * 8 + (threadIdx.x >> 5);
+  if (d.x >= 0 && r < d.w) {
+    const int pr = e.x + r;
+    join_row<D, F16>(a, 1 + d.z, [&](int p) {
+      return static_cast<int64_t>(p == 0 ? 2 * blockIdx.x + 1 : 2 * (blockIdx.x + p)) * kTileRows + r;
+    }, a.out + static_cast<int64_t>(d.x + pr / a.G) * a.o_st + static_cast<int64_t>(d.y * a.G + pr % a.G) * a.o_sh);
   }
   pdl_trigger();
 }
@@ -1133,8 +1378,8 @@ constexpr int kSplitRows = 64;  // most rows of a sequence that the split kernel
 
 struct PagedPlan {
   bool split, tile, unit_mode;
-  int split_mt, split_ctas, tile_blocks, tile_splits;
-  size_t split_o, split_ml, split_desc, tile_o, tile_ml, bytes;  // workspace offsets
+  int split_mt, split_ctas, tile_ctas;
+  size_t split_o, split_ml, split_desc, tile_o, tile_ml, tile_desc, bytes;  // workspace offsets
 };
 
 static PagedPlan paged_plan(const qik_paged_attn_args& A) {
@@ -1163,18 +1408,11 @@ static PagedPlan paged_plan(const qik_paged_attn_args& A) {
     }
   }
   if (p.tile) {
-    const int64_t by_rows = A.T * G / kTileRows + A.B, by_seq = A.B * ((max_rows + kTileRows - 1) / kTileRows);
-    p.tile_blocks = static_cast<int>(by_rows < by_seq ? by_rows : by_seq);
-    // few blocks: the keys are split over CTAs until the GPU is full, at least 4 tiles each
-    const int64_t ctas = static_cast<int64_t>(p.tile_blocks) * A.HK, tiles = (A.max_kv + kTileN - 1) / kTileN;
-    int64_t splits = ctas >= sms ? 1 : sms / ctas;
-    if (splits > tiles / 4) splits = tiles / 4;
-    p.tile_splits = splits < 1 ? 1 : static_cast<int>(splits);
-    if (p.tile_splits > 1) {
-      const size_t rows = static_cast<size_t>(p.tile_splits) * ctas * kTileRows;
-      p.tile_o = take(rows * A.D * sizeof(float));
-      p.tile_ml = take(rows * sizeof(float2));
-    }
+    p.tile_ctas = sms;
+    const size_t rows = static_cast<size_t>(2) * sms * kTileRows;
+    p.tile_o = take(rows * A.D * sizeof(float));
+    p.tile_ml = take(rows * sizeof(float2));
+    p.tile_desc = take(static_cast<size_t>(2) * sms * sizeof(int4));
   }
   p.bytes = at;
   return p;
@@ -1190,9 +1428,11 @@ static int check_paged(const qik_paged_attn_args& A) {
               "qik_paged_attention: page of %lld tokens (a power of two, 16 to 4096), %lld pages", (long long)A.page,
               (long long)A.pages);
   QIK_REQUIRE(A.W >= 0 && A.W * A.page <= (1ll << 30), "qik_paged_attention: page table of %lld columns", (long long)A.W);
-  QIK_REQUIRE(A.B * A.HK <= 0x7FFFFFFFll && A.B * A.HK * (A.W * A.page / kSplitTile + 3) <= 0x7FFFFFFFll,
-              "qik_paged_attention: %lld sequences of up to %lld keys are too much for one call", (long long)A.B,
-              (long long)(A.W * A.page));
+  // key tiles of all units are counted in 32 bits
+  const int64_t blocks = A.T * (A.HQ / A.HK) / kTileRows + A.B, keys = A.W * A.page;
+  QIK_REQUIRE(blocks * A.HK <= 0x7FFFFFFFll && blocks * A.HK * (keys / kSplitTile + 3) <= 0x7FFFFFFFll,
+              "qik_paged_attention: %lld tokens and %lld sequences of up to %lld keys are too much for one call", (long long)A.T,
+              (long long)A.B, (long long)keys);
   QIK_REQUIRE(A.max_new >= 0 && A.max_new <= A.T && A.max_kv >= 0, "qik_paged_attention: max_new %lld of %lld tokens, max_kv %lld",
               (long long)A.max_new, (long long)A.T, (long long)A.max_kv);
   QIK_REQUIRE(A.window >= 0 && A.sinks >= 0 && A.window <= 0x3FFFFFFF && A.sinks <= 0x3FFFFFFF,
@@ -1262,14 +1502,12 @@ static cudaError_t launch_paged(const qik_paged_attn_args& A, const PagedPlan& p
     if (e != cudaSuccess) return e;
     d.lo_rows = kSplitRows;
     d.hi_rows = 0x7FFFFFFF;
-    d.splits = p.tile_splits;
     d.ws_o = reinterpret_cast<float*>(ws + p.tile_o);
     d.ws_ml = reinterpret_cast<float2*>(ws + p.tile_ml);
-    const dim3 grid(static_cast<unsigned>(A.HK), static_cast<unsigned>(p.tile_blocks), static_cast<unsigned>(p.tile_splits));
-    e = launch_kernel(paged_tile_kernel<D, F16>, grid, dim3(kTileThreads), Sh::kBytes, st, true, maps[2], maps[3], d);
-    if (e != cudaSuccess || p.tile_splits == 1) return e;
-    const dim3 jgrid(static_cast<unsigned>(A.HK), static_cast<unsigned>(p.tile_blocks), 8);
-    e = launch_kernel(paged_tile_join_kernel<D, F16>, jgrid, dim3(256), 0, st, true, d);
+    d.ws_desc = reinterpret_cast<int4*>(ws + p.tile_desc);
+    e = launch_kernel(paged_tile_kernel<D, F16>, dim3(p.tile_ctas), dim3(kTileThreads), Sh::kBytes, st, true, maps[2], maps[3], d);
+    if (e != cudaSuccess) return e;
+    e = launch_kernel(paged_tile_join_kernel<D, F16>, dim3(p.tile_ctas, kTileRows / 8), dim3(256), 0, st, true, d);
   }
   return e;
 }
@@ -1299,7 +1537,6 @@ extern "C" int qik_paged_attention(const qik_paged_attn_args* args, void* ws, si
   const PagedPlan p = paged_plan(A);
   QIK_REQUIRE(p.bytes == 0 || (ws && ws_bytes >= p.bytes), "qik_paged_attention: workspace of %zu bytes, %zu needed",
               ws_bytes, p.bytes);
-  QIK_REQUIRE(p.tile_blocks <= 65535, "qik_paged_attention: %d row blocks are too many (65535)", p.tile_blocks);
   const bool f16 = (A.flags & QIK_PAGED_F16) != 0;
   CUtensorMap maps[4];
   if (p.split) {
@@ -1322,7 +1559,7 @@ extern "C" int qik_paged_attention(const qik_paged_attn_args* args, void* ws, si
   while ((1ll << d.page_log2) < A.page) ++d.page_log2;
   d.max_new = static_cast<int>(A.max_new);
   d.window = A.window, d.sinks = A.window > 0 ? A.sinks : 0;
-  d.splits = 1, d.min_share = 4;
+  d.min_share = 4;
   d.scale_log2 = A.sm_scale * 1.4426950408889634f;
   d.causal = (A.flags & QIK_PAGED_CAUSAL) != 0;
   cudaStream_t st = static_cast<cudaStream_t>(stream);

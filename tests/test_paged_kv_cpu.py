@@ -32,7 +32,13 @@ def cache(monkeypatch):
             for a, b, t in moves:
                 p[:, b, :, :t] = old[:, a, :, :t]
     monkeypatch.setattr(P, "copy_pages", plain)
-    return lambda pages=12, page=16: P.PagedKVCache(1, pages, page, 1, 8, dtype=torch.float32, device="cpu")
+
+    def make(pages=12, page=16):
+        c = P.PagedKVCache(1, pages, page, 1, 8, dtype=torch.float32, device="cpu")
+        c.k_pages.zero_()  # (a new pool holds whatever the memory held, NaN too)
+        c.v_pages.zero_()
+        return c
+    return make
 
 
 def test_step_positions_slots_and_table(cache):
