@@ -391,7 +391,7 @@ PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     r.sm_scale = static_cast<float>(scale);
     r.flags = (causal ? QIK_PAGED_CAUSAL : 0) | (q0.scalar_type() == at::kHalf ? QIK_PAGED_F16 : 0);
     c10::cuda::OptionalCUDAGuard guard(q0.device());
-    const at::Tensor q = q0.stride(2) != 1 || ((q0.stride(0) | q0.stride(1)) & 7) || !aligned(q0) ? q0.clone(at::MemoryFormat::Contiguous) : q0;
+    const at::Tensor q = q0.stride(2) != 1 || q0.stride(0) <= 0 || q0.stride(1) <= 0 || ((q0.stride(0) | q0.stride(1)) & 7) || !aligned(q0) ? q0.clone(at::MemoryFormat::Contiguous) : q0;
     const bool given = a[12] != Py_None;
     const at::Tensor o = given ? tensor(a[12], "out") : empty(q.sizes(), q.scalar_type(), q);
     if (given) {

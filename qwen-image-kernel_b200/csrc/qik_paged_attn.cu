@@ -53,6 +53,7 @@ struct PagedDev {
   int window, sinks, min_share;
   float scale_log2;
   bool causal, unit_mode;
+  int tile_tok;          // tile kernel: tokens of a 128-row query tile (128 / G)
   int lo_rows, hi_rows;  // rows (new tokens x group) of the sequences this launch takes
 };
 
@@ -695,28 +696,32 @@ struct TileShape {
   static_assert(kBytes <= 232448, "shared memory above the 227 KB per-CTA limit");
 };
 
-// A unit of this kernel is a (sequence, key head, 256-row block); its work is its key tiles.
+// A unit of this kernel is a (sequence, key head, block of two query tiles); its work is its key
+// tiles and kUnitCost more for the change to it (first q and K, first softmax, last product and
+// the stores: without it the CTAs with the many short units at a prompt's start end last).
+constexpr int kUnitCost = 3;
 struct Block {
   Seq s;
   Tiles t;
-  int i, h, rb, blocks;  // sequence, key head, row block, row blocks of the sequence
+  int i, h, rb, blocks;  // sequence, key head, block, blocks of the sequence
   int at, nt;            // tile within the unit, the unit's tiles
-  int left;              // tiles left in the CTA's range
+  int taken;             // tiles of the unit that are in the CTA's range
+  int left;              // work left in the CTA's range, this unit's not counted
 };
 __device__ __forceinline__ int row_blocks(const PagedDev& a, const Seq& s) {
   const int rows = s.n * a.G;
-  return rows > a.lo_rows ? (rows + kTileRows - 1) / kTileRows : 0;
+  return rows > a.lo_rows ? (s.n + 2 * a.tile_tok - 1) / (2 * a.tile_tok) : 0;
 }
 __device__ __forceinline__ Tiles block_tiles(const PagedDev& a, const Seq& s, int rb) {
-  const int row0 = rb * kTileRows, rows = min(s.n * a.G - row0, kTileRows);
-  return tiles_of<kTileN>(a, s, row0 / a.G, (row0 + rows - 1) / a.G + 1);
+  const int j0 = rb * 2 * a.tile_tok;
+  return tiles_of<kTileN>(a, s, j0, min(j0 + 2 * a.tile_tok, s.n));
 }
 // (a unit whose rows see no key still has one tile, so that its rows are written as zeros)
 __device__ __forceinline__ int block_work(const PagedDev& a, const Seq& s, int rb) {
   const Tiles t = block_tiles(a, s, rb);
-  return max(1, t.sink + t.main);
+  return max(1, t.sink + t.main) + kUnitCost;
 }
-// Tiles of all row blocks of the sequence of one key head.  Whole warp: lanes with few
+// Work of all row blocks of the sequence of one key head.  Whole warp: lanes with few
 // blocks add theirs up alone, the others' blocks are shared out over the warp.
 __device__ __forceinline__ int sequence_work(const PagedDev& a, const Seq& s, int blocks) {
   int sum = 0;
@@ -736,14 +741,18 @@ __device__ __forceinline__ int sequence_work(const PagedDev& a, const Seq& s, in
   }
   return sum;
 }
-__device__ __forceinline__ void open_block(const PagedDev& a, Block& b) {
+// Opens the unit at (i, h, rb) with `done` of its work (the change to it first, then its tiles) in
+// earlier CTAs' ranges; false: the range ends before a tile of it.
+__device__ __forceinline__ bool open_block(const PagedDev& a, Block& b, int done) {
   b.t = block_tiles(a, b.s, b.rb);
   b.nt = max(1, b.t.sink + b.t.main);
+  b.at = max(0, done - kUnitCost);
+  b.taken = min(b.nt, done + b.left - kUnitCost) - b.at;
+  b.left -= b.nt + kUnitCost - done;
+  return b.taken > 0;
 }
-__device__ __forceinline__ bool next_block(const PagedDev& a, Block& b, int taken) {
-  b.left -= taken;
+__device__ __forceinline__ bool next_block(const PagedDev& a, Block& b) {
   if (b.left <= 0) return false;
-  b.at = 0;
   if (++b.rb == b.blocks) {
     b.rb = 0;
     if (++b.h == a.HK) {
@@ -755,10 +764,9 @@ __device__ __forceinline__ bool next_block(const PagedDev& a, Block& b, int take
       } while (b.blocks == 0);
     }
   }
-  open_block(a, b);
-  return true;
+  return open_block(a, b, 0);
 }
-// The CTA's range of tiles: an equal share of all of them, counted sequence by sequence, head
+// The CTA's range of work: an equal share of all of it, counted sequence by sequence, head
 // by head, row block by row block.  All threads; `slot`: 32 ints of shared memory.
 __device__ __forceinline__ bool open_range(const PagedDev& a, Block& b, int& share, int* slot) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
@@ -816,7 +824,7 @@ __device__ __forceinline__ bool open_range(const PagedDev& a, Block& b, int& sha
   b.s = seq_of(a, b.i);
   b.blocks = row_blocks(a, b.s);
   int rest = slot[2];
-  for (int rb0 = 0;; rb0 += 32) {  // the row block that holds tile `rest` (every warp for itself)
+  for (int rb0 = 0;; rb0 += 32) {  // the block that holds `rest` (every warp for itself)
     const int rb = rb0 + lane;
     const int work = rb < b.blocks ? block_work(a, b.s, rb) : 0;
     int incl = work;
@@ -829,18 +837,17 @@ __device__ __forceinline__ bool open_range(const PagedDev& a, Block& b, int& sha
     if (past) {
       const int l = __ffs(past) - 1;
       b.rb = rb0 + l;
-      b.at = rest - __shfl_sync(0xffffffffu, incl - work, l);
+      rest -= __shfl_sync(0xffffffffu, incl - work, l);
       break;
     }
     rest -= __shfl_sync(0xffffffffu, incl, 31);
     if (rb0 + 32 >= b.blocks) {  // (not reached: `rest` lies in the sequence)
       b.rb = b.blocks - 1;
-      b.at = 0;
+      rest = 0;
       break;
     }
   }
-  open_block(a, b);
-  return true;
+  return open_block(a, b, rest);  // (uniform: the range may end before the unit's first tile)
 }
 
 // 32 of the D / 2 columns of O that each of a row's two threads has.
@@ -886,7 +893,7 @@ __device__ __forceinline__ float tile_softmax(const float (&sv)[64], float scale
 // What the warps know of a segment, in a ring in shared memory: kept there so that the softmax
 // threads, which hold half a score row each, have their registers for that.
 struct Segment {
-  int valid, i, q0, h, row0, rows;  // sequence, its first row of q, key head, packed rows of the block
+  int valid, i, q0, h, tok0, toks;  // sequence, its first row of q, key head, new tokens of the block
   int n, n0, n1;                    // key tiles; of them, those that query tiles 0 and 1 need
   int kv0, sink_end, main0;         // first key; where the sink tiles end and the others begin
   int lmin, lmax, offset, kv;       // keys that some row sees; place of new token 0; tokens
@@ -901,14 +908,15 @@ constexpr int kSegRing = 4;
 //   warp 0      K and V tiles by TMA into 2-stage rings, V one tile behind K;
 //   warp 1      MMA issuer (one thread): per tile t and query tile g, O_g += P_g(t) V_t, then
 //               S_g(t + 1) = Q_g K_{t+1}^T (qik_attn.cu has the ordering argument);
-//   warps 2-3   q rows of the next segment into shared memory once the last S is done; warp 2
-//               also zeroes V rows that no row of the block sees, warp 3 writes the segments;
+//   warp 2      zeroes V rows that no row of the block sees;
+//   warp 3      writes the segments; q by TMA, once the last segment's last S is done (a box is
+//               (columns, group heads, tokens), which is the packed row order);
 //   warps 4-19  softmax, eight warps per query tile, two threads a row.
 // Query tile 0 ends earlier than tile 1 under a causal mask: its count of tiles is its own.
 template <int D, bool F16>
 __global__ void __launch_bounds__(kTileThreads, 1)
     paged_tile_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
-                      const PagedDev a) {
+                      const __grid_constant__ CUtensorMap tm_q, const PagedDev a) {
   using Sh = TileShape<D>;
   constexpr int kHalfO = D / 2;  // output columns of a softmax thread
   extern __shared__ uint8_t smem_raw[];
@@ -935,7 +943,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    mbar_init(q_full, 2);
+    mbar_init(q_full, 1);
     mbar_init(q_empty, 1);
     for (int s = 0; s < 2; ++s) {
       mbar_init(&k_full[s], 1);
@@ -960,7 +968,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   Block b;
   int share;
   const bool any = open_range(a, b, share, slot);
-  if (threadIdx.x == 0) a.ws_desc[2 * blockIdx.x] = make_int4(-1, 0, 0, 0);
+  if (threadIdx.x == 0) a.ws_desc[blockIdx.x] = make_int4(-1, 0, 0, 0);
   if (!any) {
     pdl_trigger();
     return;
@@ -1119,79 +1127,17 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         base += n;
       }
     }
-  } else if (warp < 4) {
-    // ------------------------------------------------------------ q rows; V rows nobody sees
-    uint32_t base = 0, q_n = 0, seen[2] = {0u, 0u};
-    bool ok = true, more = true;
-    for (uint32_t seg = 0; ok; ++seg) {
+  } else if (warp == 2) {
+    // ------------------------------------------------------------ V rows nobody sees
+    uint32_t base = 0, seen[2] = {0u, 0u};
+    bool ok = true;
+    for (uint32_t seg = 0; ok && __all_sync(0xffffffffu, seg_wait(seg)); ++seg) {
       volatile Segment* sg = ring + (seg & (kSegRing - 1));
-      if (warp == 3) {  // writes the segment (or the end)
-        if (seg >= kSegRing)
-          ok = __all_sync(0xffffffffu, mbar_wait(&seg_empty[seg & (kSegRing - 1)], (seg / kSegRing - 1) & 1, abort_flag, a.status));
-        if (!ok) break;
-        if (lane == 0) {
-          sg->valid = more;
-          if (more) {
-            const int rows = min(b.s.n * a.G - b.rb * kTileRows, kTileRows), row0 = b.rb * kTileRows;
-            const int taken = min(b.nt - b.at, b.left), n = b.t.main == 0 ? 0 : taken;
-            const int last = last_key(a, b.s, (row0 + min(rows, kTileM) - 1) / a.G);
-            sg->i = b.i, sg->q0 = b.s.q0, sg->h = b.h, sg->row0 = row0, sg->rows = rows;
-            sg->n = n;
-            sg->n0 = last < 0 ? 0 : max(0, min(n, b.t.sink + last / kTileN - b.t.t0 + 1 - b.at));
-            sg->n1 = rows > kTileM ? n : 0;
-            sg->kv0 = tile_at(b.t, b.at) * kTileN;
-            sg->sink_end = b.t.sink > 0 ? b.t.sink * kTileN : -1;
-            sg->main0 = b.t.t0 * kTileN;
-            sg->lmin = b.t.lmin, sg->lmax = b.t.lmax, sg->kv = b.s.kv;
-            sg->offset = b.s.kv - b.s.n;
-            sg->begins = b.at == 0, sg->ends = b.at + taken == b.nt;
-            sg->pieces = (b.nt - b.at - taken + share - 1) / share;
-          }
-          mbar_arrive(&seg_full[seg & (kSegRing - 1)]);
-        }
-        __syncwarp();
-        if (!more) break;
-        more = next_block(a, b, min(b.nt - b.at, b.left));
-      } else {
-        ok = __all_sync(0xffffffffu, seg_wait(seg));
-        if (!ok) break;
-      }
-      const int n = sg->n, rows = sg->rows, row0 = sg->row0, q0 = sg->q0, h = sg->h, lmin = sg->lmin, lmax = sg->lmax,
-                sink_end = sg->sink_end, main0 = sg->main0;
+      const int n = sg->n, lmin = sg->lmin, lmax = sg->lmax, sink_end = sg->sink_end, main0 = sg->main0;
       int kv0 = sg->kv0;
       __syncwarp();
-      if (warp == 2 && lane == 0) mbar_arrive(&seg_empty[seg & (kSegRing - 1)]);
-      if (n == 0) continue;
-      if (q_n > 0) ok = __all_sync(0xffffffffu, mbar_wait(q_empty, (q_n - 1) & 1, abort_flag, a.status));
-      if (!ok) break;
-      ++q_n;
-      {  // a thread has one 16-byte chunk of every kStep-th row
-        constexpr int kChunks = D / 8, kStep = 64 / kChunks;
-        const int n_rows = rows > kTileM ? kTileRows : kTileM;
-        const int x = threadIdx.x - 64, ch = x % kChunks;
-        int r = x / kChunks;
-        const int pr = row0 + r, j = pr / a.G;
-        int gg = pr % a.G;
-        const int dj = kStep / a.G, dg = kStep % a.G;
-        const uint16_t* src = a.q + static_cast<int64_t>(q0 + j) * a.q_st + static_cast<int64_t>(h * a.G + gg) * a.q_sh + ch * 8;
-        const int64_t step = dj * a.q_st + dg * a.q_sh, wrap = a.q_st - a.G * a.q_sh;
-        const uint32_t dst = smem_u32(sQ) + (ch >> 3) * Sh::kHalfBytes;
-        for (; r < n_rows; r += kStep) {
-          const int rr = r & 127;
-          cp_async16(dst + (r >> 7) * Sh::kOperand + rr * 128 + (((ch & 7) ^ (rr & 7)) << 4), r < rows ? src : a.q, r < rows);
-          src += step;
-          gg += dg;
-          if (gg >= a.G) {
-            gg -= a.G;
-            src += wrap;
-          }
-        }
-        cp_async_wait_all();
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(q_full);
-      }
-      for (int t = 0; t < n && warp == 2; ++t) {
+      if (lane == 0) mbar_arrive(&seg_empty[seg & (kSegRing - 1)]);
+      for (int t = 0; t < n; ++t) {
         const int st = (base + t) & 1;
         if (edge(kv0, lmin, lmax)) {
           ok = __all_sync(0xffffffffu, mbar_wait(&v_raw[st], seen[st]++ & 1u, abort_flag, a.status));
@@ -1213,13 +1159,56 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       }
       base += n;
     }
+  } else if (warp == 3) {
+    // ------------------------------------------------------------ segments and q
+    if (lane == 0) {
+      uint32_t q_n = 0;
+      bool ok = true, more = true;
+      for (uint32_t seg = 0; ok; ++seg) {
+        volatile Segment* sg = ring + (seg & (kSegRing - 1));
+        if (seg >= kSegRing) ok = mbar_wait(&seg_empty[seg & (kSegRing - 1)], (seg / kSegRing - 1) & 1, abort_flag, a.status);
+        if (!ok) break;
+        const int tok0 = b.rb * 2 * a.tile_tok, toks = min(b.s.n - tok0, 2 * a.tile_tok), n = b.t.main == 0 ? 0 : b.taken;
+        sg->valid = more;
+        if (more) {
+          const int last = last_key(a, b.s, tok0 + min(toks, a.tile_tok) - 1);
+          sg->i = b.i, sg->q0 = b.s.q0, sg->h = b.h, sg->tok0 = tok0, sg->toks = toks;
+          sg->n = n;
+          sg->n0 = last < 0 ? 0 : max(0, min(n, b.t.sink + last / kTileN - b.t.t0 + 1 - b.at));
+          sg->n1 = toks > a.tile_tok ? n : 0;
+          sg->kv0 = tile_at(b.t, b.at) * kTileN;
+          sg->sink_end = b.t.sink > 0 ? b.t.sink * kTileN : -1;
+          sg->main0 = b.t.t0 * kTileN;
+          sg->lmin = b.t.lmin, sg->lmax = b.t.lmax, sg->kv = b.s.kv;
+          sg->offset = b.s.kv - b.s.n;
+          sg->begins = b.at == 0, sg->ends = b.at + b.taken == b.nt;
+          sg->pieces = (b.nt - b.at - b.taken + share - 1) / share;
+        }
+        mbar_arrive(&seg_full[seg & (kSegRing - 1)]);
+        if (!more) break;
+        if (n > 0) {
+          if (q_n > 0) ok = mbar_wait(q_empty, (q_n - 1) & 1, abort_flag, a.status);
+          if (!ok) break;
+          ++q_n;
+          const int tiles = toks > a.tile_tok ? 2 : 1;
+          mbar_arrive_expect_tx(q_full, tiles * Sh::kHalves * a.tile_tok * a.G * 128);
+          for (int g = 0; g < tiles; ++g)
+            for (int hd = 0; hd < Sh::kHalves; ++hd)
+              tma_load_4d(sQ + g * Sh::kOperand + hd * Sh::kHalfBytes, &tm_q, 0, b.h * a.G, b.s.q0 + tok0 + g * a.tile_tok, hd, q_full);
+        }
+        more = next_block(a, b);
+      }
+    }
   } else {
     // ------------------------------------------------------------ softmax (tile g)
     const int g = (warp - 4) >> 3;
     const int hc = lane >> 4;  // column half of the row
     // TMEM lane quarter warp % 4, its lower or upper 16 lanes by (warp / 4) % 2
     const int lane0 = (warp & 3) * 32 + (((warp - 4) >> 2) & 1) * 16;
-    const int r = g * kTileM + lane0 + (lane & 15);
+    // the row's place in its query tile: token r / G of the tile, head r % G of the group; rows that
+    // hold none (behind the last token, or the 128 % G last) follow another and are not stored
+    const int r = lane0 + (lane & 15);
+    const int tok = min(r / a.G, a.tile_tok - 1) + g * a.tile_tok;
     const uint32_t tS = tmem + (static_cast<uint32_t>(lane0) << 16) + 128u * g;
     const uint32_t tO = tS + 256u;
     uint32_t s_n = 0, o_n = 0;  // S tiles and segments of this query tile so far
@@ -1229,7 +1218,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       const int work = g == 0 ? sg->n0 : sg->n1;
       int my_last, my_first, kv0 = sg->kv0;
       {
-        const int j = (sg->row0 + min(r, sg->rows - 1)) / a.G;  // rows behind the last follow it, unstored
+        const int j = sg->tok0 + min(tok, sg->toks - 1);
         my_last = a.causal ? sg->offset + j : sg->kv - 1;
         my_first = first_key(a, my_last);
       }
@@ -1304,12 +1293,12 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       if (work > 0 && ok) ok = __all_sync(0xffffffffu, mbar_wait(&o_full[g], o_n++ & 1, abort_flag, a.status));
       if (!ok) break;
       tc_fence_after();
-      const int rows = sg->rows, pr = sg->row0 + r;
+      const bool stored = r < a.tile_tok * a.G && tok < sg->toks;
       const bool whole = sg->begins && sg->ends;
       const float inv = !whole ? 1.0f : l_row == 0.0f ? 0.0f : 1.0f / l_row;
-      uint16_t* dst = a.out + static_cast<int64_t>(sg->q0 + pr / a.G) * a.o_st +
-                      static_cast<int64_t>(sg->h * a.G + pr % a.G) * a.o_sh + kHalfO * hc;
-      const int64_t at = static_cast<int64_t>(2 * blockIdx.x + (sg->begins ? 1 : 0)) * kTileRows + r;
+      uint16_t* dst = a.out + static_cast<int64_t>(sg->q0 + sg->tok0 + tok) * a.o_st +
+                      static_cast<int64_t>(sg->h * a.G + r % a.G) * a.o_sh + kHalfO * hc;
+      const int64_t at = static_cast<int64_t>(2 * blockIdx.x + (sg->begins ? 1 : 0)) * kTileRows + g * kTileM + r;
 #pragma unroll
       for (int c = 0; c < D / 64; ++c) {
         uint32_t o[32];
@@ -1324,7 +1313,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           __syncwarp();
           if (lane == 0) mbar_arrive(&o_empty[g]);
         }
-        if (r < rows && whole) {
+        if (stored && whole) {
 #pragma unroll
           for (int i = 0; i < 32; i += 8) {
             uint32_t w[4];
@@ -1333,16 +1322,15 @@ __global__ void __launch_bounds__(kTileThreads, 1)
               w[k] = pack16<F16>(__uint_as_float(o[i + 2 * k]) * inv, __uint_as_float(o[i + 2 * k + 1]) * inv);
             *reinterpret_cast<uint4*>(dst + c * 32 + i) = make_uint4(w[0], w[1], w[2], w[3]);
           }
-        } else if (r < rows) {
+        } else if (stored) {
           uint4* part = reinterpret_cast<uint4*>(a.ws_o + at * D + kHalfO * hc + c * 32);
 #pragma unroll
           for (int i = 0; i < 8; ++i) part[i] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
         }
       }
-      if (r < rows && !whole && hc == 0) a.ws_ml[at] = make_float2(m_run, l_row);
+      if (stored && !whole && hc == 0) a.ws_ml[at] = make_float2(m_run, l_row);
       if (warp == 4 && lane == 0 && sg->begins && !sg->ends) {
-        a.ws_desc[2 * blockIdx.x] = make_int4(sg->q0, sg->h, sg->pieces, rows);
-        a.ws_desc[2 * blockIdx.x + 1] = make_int4(sg->row0, 0, 0, 0);
+        a.ws_desc[blockIdx.x] = make_int4(sg->q0 + sg->tok0, sg->h, sg->pieces, sg->toks);
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&seg_empty[seg & (kSegRing - 1)]);
@@ -1362,14 +1350,13 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 template <int D, bool F16>
 __global__ void __launch_bounds__(256) paged_tile_join_kernel(const PagedDev a) {
   pdl_wait();
-  const int4 d = __ldcg(a.ws_desc + 2 * blockIdx.x), e = __ldcg(a.ws_desc + 2 * blockIdx.x + 1);
-  const int r = blockIdx.y * 8 + (threadIdx.x >> 5);
-  if (d.x >= 0 && r < d.w) {
-    const int pr = e.x + r;
+  const int4 d = __ldcg(a.ws_desc + blockIdx.x);  // first row of q, head, further pieces, tokens
+  const int g = blockIdx.y >> 4, r = (blockIdx.y & 15) * 8 + (threadIdx.x >> 5);
+  const int tok = r / a.G + g * a.tile_tok;
+  if (d.x >= 0 && r < a.tile_tok * a.G && tok < d.w)
     join_row<D, F16>(a, 1 + d.z, [&](int p) {
-      return static_cast<int64_t>(p == 0 ? 2 * blockIdx.x + 1 : 2 * (blockIdx.x + p)) * kTileRows + r;
-    }, a.out + static_cast<int64_t>(d.x + pr / a.G) * a.o_st + static_cast<int64_t>(d.y * a.G + pr % a.G) * a.o_sh);
-  }
+      return static_cast<int64_t>(p == 0 ? 2 * blockIdx.x + 1 : 2 * (blockIdx.x + p)) * kTileRows + g * kTileM + r;
+    }, a.out + static_cast<int64_t>(d.x + tok) * a.o_st + static_cast<int64_t>(d.y * a.G + r % a.G) * a.o_sh);
   pdl_trigger();
 }
 
@@ -1412,7 +1399,7 @@ static PagedPlan paged_plan(const qik_paged_attn_args& A) {
     const size_t rows = static_cast<size_t>(2) * sms * kTileRows;
     p.tile_o = take(rows * A.D * sizeof(float));
     p.tile_ml = take(rows * sizeof(float2));
-    p.tile_desc = take(static_cast<size_t>(2) * sms * sizeof(int4));
+    p.tile_desc = take(sms * sizeof(int4));
   }
   p.bytes = at;
   return p;
@@ -1429,8 +1416,9 @@ static int check_paged(const qik_paged_attn_args& A) {
               (long long)A.pages);
   QIK_REQUIRE(A.W >= 0 && A.W * A.page <= (1ll << 30), "qik_paged_attention: page table of %lld columns", (long long)A.W);
   // key tiles of all units are counted in 32 bits
-  const int64_t blocks = A.T * (A.HQ / A.HK) / kTileRows + A.B, keys = A.W * A.page;
-  QIK_REQUIRE(blocks * A.HK <= 0x7FFFFFFFll && blocks * A.HK * (keys / kSplitTile + 3) <= 0x7FFFFFFFll,
+  QIK_REQUIRE(A.HQ / A.HK <= 64, "qik_paged_attention: %lld query heads of one key head (64)", (long long)(A.HQ / A.HK));
+  const int64_t blocks = A.T / (kTileM / (A.HQ / A.HK)) + A.B, keys = A.W * A.page;
+  QIK_REQUIRE(blocks * A.HK <= 0x7FFFFFFFll && blocks * A.HK * (keys / kSplitTile + 3 + kUnitCost) <= 0x7FFFFFFFll,
               "qik_paged_attention: %lld tokens and %lld sequences of up to %lld keys are too much for one call", (long long)A.T,
               (long long)A.B, (long long)keys);
   QIK_REQUIRE(A.max_new >= 0 && A.max_new <= A.T && A.max_kv >= 0, "qik_paged_attention: max_new %lld of %lld tokens, max_kv %lld",
@@ -1505,7 +1493,7 @@ static cudaError_t launch_paged(const qik_paged_attn_args& A, const PagedPlan& p
     d.ws_o = reinterpret_cast<float*>(ws + p.tile_o);
     d.ws_ml = reinterpret_cast<float2*>(ws + p.tile_ml);
     d.ws_desc = reinterpret_cast<int4*>(ws + p.tile_desc);
-    e = launch_kernel(paged_tile_kernel<D, F16>, dim3(p.tile_ctas), dim3(kTileThreads), Sh::kBytes, st, true, maps[2], maps[3], d);
+    e = launch_kernel(paged_tile_kernel<D, F16>, dim3(p.tile_ctas), dim3(kTileThreads), Sh::kBytes, st, true, maps[2], maps[3], maps[4], d);
     if (e != cudaSuccess) return e;
     e = launch_kernel(paged_tile_join_kernel<D, F16>, dim3(p.tile_ctas, kTileRows / 8), dim3(256), 0, st, true, d);
   }
@@ -1532,13 +1520,13 @@ extern "C" int qik_paged_attention(const qik_paged_attn_args* args, void* ws, si
   QIK_REQUIRE(aligned16(A.q) && aligned16(A.out) && aligned16(A.k_pages) && aligned16(A.v_pages) && aligned16(ws),
               "qik_paged_attention: q, out, pages and workspace must be 16-byte aligned");
   QIK_REQUIRE((A.q_st | A.q_sh | A.o_st | A.o_sh | A.kp_s0 | A.kp_sh | A.kp_ss | A.vp_s0 | A.vp_sh | A.vp_ss) % 8 == 0 &&
-                  A.kp_s0 >= 0 && A.kp_sh >= 0 && A.kp_ss > 0 && A.vp_s0 >= 0 && A.vp_sh >= 0 && A.vp_ss > 0,
+                  A.q_st > 0 && A.q_sh > 0 && A.kp_s0 >= 0 && A.kp_sh >= 0 && A.kp_ss > 0 && A.vp_s0 >= 0 && A.vp_sh >= 0 && A.vp_ss > 0,
               "qik_paged_attention: strides must be multiples of 8 elements");
   const PagedPlan p = paged_plan(A);
   QIK_REQUIRE(p.bytes == 0 || (ws && ws_bytes >= p.bytes), "qik_paged_attention: workspace of %zu bytes, %zu needed",
               ws_bytes, p.bytes);
   const bool f16 = (A.flags & QIK_PAGED_F16) != 0;
-  CUtensorMap maps[4];
+  CUtensorMap maps[5];
   if (p.split) {
     rc = page_map(&maps[0], A.k_pages, f16, A, A.kp_s0, A.kp_sh, A.kp_ss, kSplitTile, static_cast<uint32_t>(A.D / 64));
     if (!rc) rc = page_map(&maps[1], A.v_pages, f16, A, A.vp_s0, A.vp_sh, A.vp_ss, kSplitTile, static_cast<uint32_t>(A.D / 64));
@@ -1546,6 +1534,13 @@ extern "C" int qik_paged_attention(const qik_paged_attn_args* args, void* ws, si
   if (!rc && p.tile) {
     rc = page_map(&maps[2], A.k_pages, f16, A, A.kp_s0, A.kp_sh, A.kp_ss, kTileN, 1);
     if (!rc) rc = page_map(&maps[3], A.v_pages, f16, A, A.vp_s0, A.vp_sh, A.vp_ss, kTileN, 1);
+    if (!rc) {  // q: (64 columns, head, token, half), boxes of a group's heads and a query tile's tokens
+      const uint64_t dims[4] = {64, static_cast<uint64_t>(A.HQ), static_cast<uint64_t>(A.T), static_cast<uint64_t>(A.D / 64)};
+      const uint64_t strides[3] = {static_cast<uint64_t>(A.q_sh * 2), static_cast<uint64_t>(A.q_st * 2), 128};
+      const uint32_t group = static_cast<uint32_t>(A.HQ / A.HK), box[4] = {64, group, 128 / group, 1};
+      rc = make_tmap_nd(&maps[4], A.q, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, dims,
+                        strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+    }
   }
   if (rc) return rc;
   PagedDev d = {};
@@ -1558,6 +1553,7 @@ extern "C" int qik_paged_attention(const qik_paged_attn_args* args, void* ws, si
   d.G = static_cast<int>(A.HQ / A.HK), d.W = static_cast<int>(A.W), d.pages = static_cast<int>(A.pages);
   while ((1ll << d.page_log2) < A.page) ++d.page_log2;
   d.max_new = static_cast<int>(A.max_new);
+  d.tile_tok = 128 / d.G;
   d.window = A.window, d.sinks = A.window > 0 ? A.sinks : 0;
   d.min_share = 4;
   d.scale_log2 = A.sm_scale * 1.4426950408889634f;
