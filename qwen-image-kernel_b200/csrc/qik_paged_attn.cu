@@ -19,7 +19,7 @@
 //   ragged batches and a single long sequence fill the GPU alike; every CTA finds its
 //   range from the lengths on the device (the host needs none of them, a captured graph
 //   follows them).  A (sequence, head) that one CTA covers is finished there; pieces go
-//   to a workspace and are joined by paged_split_join_kernel in a fixed order.  Two
+//   to a workspace and are joined by paged_join_kernel in a fixed order.  Two
 //   TMA warps fill a ring of K and V tiles; 8 warps split the tiles, their keys and the
 //   16-row groups between them and run mma.sync m16n8k16: tcgen05's 128-row tiles would be
 //   8 to 87% padding here and the tensor pipe is not what bounds it.
@@ -606,64 +606,6 @@ __global__ void __launch_bounds__(SplitShape<D, MT, TEAMS>::kThreads, SplitShape
       more = walk_next(a, w, count);
     }
   }
-  pdl_trigger();
-}
-
-// sum_p f_p o_p / sum_p f_p l_p, f_p = 2^(m_p - max m), over the pieces of one row: `at(p)` is
-// piece p's row in the workspace.  One warp; lane holds D / 32 columns.  Pieces are added in
-// order, four loads in flight.
-template <int D, bool F16, typename At>
-__device__ __forceinline__ void join_row(const PagedDev& a, int pieces, At at, uint16_t* dst) {
-  using Vec = typename std::conditional<D == 128, float4, float2>::type;
-  const int lane = threadIdx.x & 31;
-  float top = -INFINITY, sum = 0.0f;
-  for (int p = lane; p < pieces; p += 32) top = fmaxf(top, __ldcg(a.ws_ml + at(p)).x);
-  float acc[D / 32];
-#pragma unroll
-  for (int c = 0; c < D / 32; ++c) acc[c] = 0.0f;
-  for (int p0 = 0; p0 < pieces; p0 += 4) {
-    float2 ml[4];
-    Vec v[4];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int64_t row = at(min(p0 + k, pieces - 1));
-      ml[k] = __ldcg(a.ws_ml + row);
-      v[k] = __ldcg(reinterpret_cast<const Vec*>(a.ws_o + row * D) + lane);
-    }
-    if (p0 == 0) {
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    }
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const float f = p0 + k >= pieces || ml[k].x == -INFINITY ? 0.0f : ex2(ml[k].x - top);
-      if (p0 + k < pieces) {
-        sum = fmaf(ml[k].y, f, sum);
-        const float* e = reinterpret_cast<const float*>(&v[k]);
-#pragma unroll
-        for (int c = 0; c < D / 32; ++c) acc[c] = fmaf(e[c], f, acc[c]);
-      }
-    }
-  }
-  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-  if constexpr (D == 128)
-    reinterpret_cast<uint2*>(dst)[lane] =
-        make_uint2(pack16<F16>(acc[0] * inv, acc[1] * inv), pack16<F16>(acc[2] * inv, acc[3] * inv));
-  else
-    reinterpret_cast<uint32_t*>(dst)[lane] = pack16<F16>(acc[0] * inv, acc[1] * inv);
-}
-
-// Joins the pieces of the unit that CTA blockIdx.x of the split kernel left open: its own
-// piece, then the following CTAs' first pieces.  Four rows a CTA.
-template <int D, bool F16>
-__global__ void __launch_bounds__(128) paged_split_join_kernel(const PagedDev a, int slot_rows) {
-  pdl_wait();
-  const int4 d = __ldcg(a.ws_desc + blockIdx.x);  // first new token, head, further pieces, rows
-  const int r = blockIdx.y * 4 + (threadIdx.x >> 5);
-  if (d.x >= 0 && r < d.w)
-    join_row<D, F16>(a, 1 + d.z, [&](int p) {
-      return static_cast<int64_t>(p == 0 ? 2 * blockIdx.x + 1 : 2 * (blockIdx.x + p)) * slot_rows + r;
-    }, a.out + static_cast<int64_t>(d.x + r / a.G) * a.o_st + static_cast<int64_t>(d.y * a.G + r % a.G) * a.o_sh);
   pdl_trigger();
 }
 
@@ -1345,18 +1287,112 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   }
 }
 
-// Joins the pieces of the unit that CTA blockIdx.x of the tile kernel left open: its own piece,
-// then the following CTAs' first pieces.  Eight rows a CTA.
+// ============================================================ joining pieces
+// out = sum_p f_p o_p / sum_p f_p l_p, f_p = 2^(m_p - max m), over the pieces of a unit that CTA
+// `cta` left open: its own, then the following CTAs' first ones, added in that order.  One warp
+// has kJoinRows rows; the first two pieces (mostly all there are) are loaded with their maxima.
+// Small CTAs and few registers: this kernel is a chain of three memory latencies (the unit, its
+// pieces, the stores) and is over sooner the more of its warps are resident.
+constexpr int kJoinRows = 2;
+constexpr int kJoinWarps = 2;
+
+struct JoinSet {  // one kernel's pieces
+  const float* o;
+  const float2* ml;
+  const int4* desc;
+  int ctas, rows, blocks;  // its CTAs, rows of a piece, join CTAs for each of its CTAs
+};
+struct JoinDev {
+  uint16_t* out;
+  int64_t o_st, o_sh;
+  int G, tile_tok;
+  JoinSet split, tile;
+};
 template <int D, bool F16>
-__global__ void __launch_bounds__(256) paged_tile_join_kernel(const PagedDev a) {
+__global__ void __launch_bounds__(kJoinWarps * 32, 16) paged_join_kernel(const JoinDev a) {
+  using Vec = typename std::conditional<D == 128, float4, float2>::type;
+  // the tile kernel's units first (they are the larger)
+  const int lane = threadIdx.x & 31, tile_blocks = a.tile.ctas * a.tile.blocks;
+  const bool toks = static_cast<int>(blockIdx.x) < tile_blocks;  // rows counted in query tiles of 128
+  const int block = toks ? blockIdx.x : blockIdx.x - tile_blocks, blocks = toks ? a.tile.blocks : a.split.blocks;
+  const float* ws_o = toks ? a.tile.o : a.split.o;
+  const float2* ws_ml = toks ? a.tile.ml : a.split.ml;
+  const int slot_rows = toks ? a.tile.rows : a.split.rows;
+  const int cta = block / blocks, r0 = (block % blocks * kJoinWarps + (threadIdx.x >> 5)) * kJoinRows;
   pdl_wait();
-  const int4 d = __ldcg(a.ws_desc + blockIdx.x);  // first row of q, head, further pieces, tokens
-  const int g = blockIdx.y >> 4, r = (blockIdx.y & 15) * 8 + (threadIdx.x >> 5);
-  const int tok = r / a.G + g * a.tile_tok;
-  if (d.x >= 0 && r < a.tile_tok * a.G && tok < d.w)
-    join_row<D, F16>(a, 1 + d.z, [&](int p) {
-      return static_cast<int64_t>(p == 0 ? 2 * blockIdx.x + 1 : 2 * (blockIdx.x + p)) * kTileRows + g * kTileM + r;
-    }, a.out + static_cast<int64_t>(d.x + tok) * a.o_st + static_cast<int64_t>(d.y * a.G + r % a.G) * a.o_sh);
+  const int4 d = __ldcg((toks ? a.tile.desc : a.split.desc) + cta);  // first row of q, head, further pieces, rows (tokens)
+  uint16_t* dst[kJoinRows];
+  bool any = false;
+#pragma unroll
+  for (int k = 0; k < kJoinRows; ++k) {
+    const int r = r0 + k;
+    const int in = toks ? r % kTileM : r, tok = toks ? in / a.G + r / kTileM * a.tile_tok : r / a.G;
+    const bool mine = d.x >= 0 && (toks ? in < a.tile_tok * a.G && tok < d.w : r < d.w);
+    any = any || mine;
+    dst[k] = mine ? a.out + static_cast<int64_t>(d.x + tok) * a.o_st + static_cast<int64_t>(d.y * a.G + in % a.G) * a.o_sh : nullptr;
+  }
+  if (any) {
+    const int pieces = 1 + d.z;
+    auto at = [&](int p, int k) { return static_cast<int64_t>(p == 0 ? 2 * cta + 1 : 2 * (cta + p)) * slot_rows + r0 + k; };
+    float2 ml[2][kJoinRows];
+    Vec v[2][kJoinRows];
+    float top[kJoinRows], sum[kJoinRows], acc[kJoinRows][D / 32];
+#pragma unroll
+    for (int p = 0; p < 2; ++p)
+#pragma unroll
+      for (int k = 0; k < kJoinRows; ++k) {
+        ml[p][k] = __ldcg(ws_ml + at(p, k));
+        v[p][k] = __ldcg(reinterpret_cast<const Vec*>(ws_o + at(p, k) * D) + lane);
+      }
+#pragma unroll
+    for (int k = 0; k < kJoinRows; ++k) {
+      top[k] = fmaxf(ml[0][k].x, ml[1][k].x);
+      if (pieces > 2) {
+        for (int p = 2 + lane; p < pieces; p += 32) top[k] = fmaxf(top[k], __ldcg(ws_ml + at(p, k)).x);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], o));
+      }
+      sum[k] = 0.0f;
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c) acc[k][c] = 0.0f;
+    }
+    auto add = [&](int k, float2 e, const Vec& o) {
+      const float f = e.x == -INFINITY ? (e.y == 0.0f ? 0.0f : 1.0f) : ex2(e.x - top[k]);  // (no key seen: 0, or NaN)
+      sum[k] = fmaf(e.y, f, sum[k]);
+      const float* x = reinterpret_cast<const float*>(&o);
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c) acc[k][c] = fmaf(x[c], f, acc[k][c]);
+    };
+#pragma unroll
+    for (int p = 0; p < 2; ++p)
+#pragma unroll
+      for (int k = 0; k < kJoinRows; ++k) add(k, ml[p][k], v[p][k]);
+    for (int p0 = 2; p0 < pieces; p0 += 2) {
+#pragma unroll
+      for (int p = 0; p < 2; ++p)
+#pragma unroll
+        for (int k = 0; k < kJoinRows; ++k)
+          if (p0 + p < pieces) {
+            ml[p][k] = __ldcg(ws_ml + at(p0 + p, k));
+            v[p][k] = __ldcg(reinterpret_cast<const Vec*>(ws_o + at(p0 + p, k) * D) + lane);
+          }
+#pragma unroll
+      for (int p = 0; p < 2; ++p)
+#pragma unroll
+        for (int k = 0; k < kJoinRows; ++k)
+          if (p0 + p < pieces) add(k, ml[p][k], v[p][k]);
+    }
+#pragma unroll
+    for (int k = 0; k < kJoinRows; ++k) {
+      const float inv = sum[k] == 0.0f ? 0.0f : 1.0f / sum[k];
+      if (!dst[k]) continue;
+      if constexpr (D == 128)
+        reinterpret_cast<uint2*>(dst[k])[lane] = make_uint2(pack16<F16>(acc[k][0] * inv, acc[k][1] * inv),
+                                                            pack16<F16>(acc[k][2] * inv, acc[k][3] * inv));
+      else
+        reinterpret_cast<uint32_t*>(dst[k])[lane] = pack16<F16>(acc[k][0] * inv, acc[k][1] * inv);
+    }
+  }
   pdl_trigger();
 }
 
@@ -1460,9 +1496,7 @@ static cudaError_t launch_split(const CUtensorMap& tk, const CUtensorMap& tv, co
   static std::once_flag once[64];
   cudaError_t e = allow_smem(paged_split_kernel<D, MT, TEAMS, F16>, Sh::kBytes, once);
   if (e != cudaSuccess) return e;
-  e = launch_kernel(paged_split_kernel<D, MT, TEAMS, F16>, dim3(ctas), dim3(Sh::kThreads), Sh::kBytes, st, true, tk, tv, d);
-  if (e != cudaSuccess || d.unit_mode) return e;
-  return launch_kernel(paged_split_join_kernel<D, F16>, dim3(ctas, MT * 4), dim3(128), 0, st, true, d, MT * 16);
+  return launch_kernel(paged_split_kernel<D, MT, TEAMS, F16>, dim3(ctas), dim3(Sh::kThreads), Sh::kBytes, st, true, tk, tv, d);
 }
 template <int D, bool F16>
 static cudaError_t launch_paged(const qik_paged_attn_args& A, const PagedPlan& p, PagedDev d, uint8_t* ws,
@@ -1493,10 +1527,21 @@ static cudaError_t launch_paged(const qik_paged_attn_args& A, const PagedPlan& p
     d.ws_o = reinterpret_cast<float*>(ws + p.tile_o);
     d.ws_ml = reinterpret_cast<float2*>(ws + p.tile_ml);
     d.ws_desc = reinterpret_cast<int4*>(ws + p.tile_desc);
-    e = launch_kernel(paged_tile_kernel<D, F16>, dim3(p.tile_ctas), dim3(kTileThreads), Sh::kBytes, st, true, maps[2], maps[3], maps[4], d);
+    e = launch_kernel(paged_tile_kernel<D, F16>, dim3(p.tile_ctas), dim3(kTileThreads), Sh::kBytes, st, true, maps[2], maps[3],
+                      maps[4], d);
     if (e != cudaSuccess) return e;
-    e = launch_kernel(paged_tile_join_kernel<D, F16>, dim3(p.tile_ctas, kTileRows / 8), dim3(256), 0, st, true, d);
   }
+  // one join for both kernels' pieces
+  JoinDev j = {d.out, d.o_st, d.o_sh, d.G, d.tile_tok, {}, {}};
+  const auto set = [&](size_t o, size_t ml, size_t desc, int ctas, int rows) {
+    return JoinSet{reinterpret_cast<const float*>(ws + o), reinterpret_cast<const float2*>(ws + ml),
+                   reinterpret_cast<const int4*>(ws + desc), ctas, rows, rows / (kJoinRows * kJoinWarps)};
+  };
+  if (p.split && !p.unit_mode) j.split = set(p.split_o, p.split_ml, p.split_desc, p.split_ctas, p.split_mt * 16);
+  if (p.tile) j.tile = set(p.tile_o, p.tile_ml, p.tile_desc, p.tile_ctas, kTileRows);
+  const int blocks = j.split.ctas * j.split.blocks + j.tile.ctas * j.tile.blocks;
+  if (blocks > 0)
+    e = launch_kernel(paged_join_kernel<D, F16>, dim3(blocks), dim3(kJoinWarps * 32), 0, st, true, j);
   return e;
 }
 
