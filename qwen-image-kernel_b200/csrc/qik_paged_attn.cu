@@ -29,9 +29,12 @@
 //
 // Pages are fetched by TMA through a 5-D map (columns, place, half, head, page): an index outside the
 // pool reads zeros, so a bad page table cannot fault; it is reported in the status word.
-// V rows that no row of the tile sees (behind the last token, before the window) are
-// zeroed in shared memory before the product: whatever an unused place of a page holds,
-// NaN too, meets p = 0 there and would spread otherwise.
+// A masked key has p = 0, and 0 x NaN would still spread through the product.  V rows that no row
+// of the tile sees (behind the last token, before the window) are zeroed in shared memory,
+// whatever an unused place of a page holds.  Where a row's result is not finite and a key that
+// it does not see, but other rows of its tile do, has infinities or NaN in V, the row is computed
+// again from the keys that it sees (mend_row, a path that finite values never take): a row's
+// result depends on what it sees alone.
 #include <mutex>
 #include <type_traits>
 
@@ -41,7 +44,7 @@
 namespace qik {
 
 struct PagedDev {
-  const uint16_t* q;
+  const uint16_t *q, *k_pages, *v_pages;
   uint16_t* out;
   const int32_t *table, *lens, *starts;
   float* ws_o;        // partial outputs
@@ -49,6 +52,7 @@ struct PagedDev {
   int4* ws_desc;      // each CTA's open unit
   int* status;
   int64_t q_st, q_sh, o_st, o_sh, table_st;
+  int64_t kp_s0, kp_sh, kp_ss, vp_s0, vp_sh, vp_ss;  // page strides (mend_row; TMA has its maps)
   int B, T, HK, G, W, pages, page_log2, max_new;
   int window, sinks, min_share;
   float scale_log2;
@@ -103,6 +107,78 @@ __device__ __forceinline__ Tiles tiles_of(const PagedDev& a, const Seq& s, int j
   return t;
 }
 __device__ __forceinline__ int tile_at(const Tiles& t, int u) { return u < t.sink ? u : t.t0 + u - t.sink; }
+
+template <bool F16>
+__device__ __forceinline__ float to_float(uint32_t half) {
+  return F16 ? __half2float(__ushort_as_half(static_cast<unsigned short>(half))) : __uint_as_float(half << 16);
+}
+// A row whose sums o (NC pairs of columns, the first two at `col`, the next ones `step` columns on,
+// in units of 2^m) are not all finite: if some key of the tiles [u0, u1) that the row does not see
+// and that is not zeroed for all rows has infinities or NaN in V, the sums are formed again, key
+// by key, from those that it sees.  Whatever else makes a sum infinite or NaN stays.
+template <int D, bool F16, int TILE, int NC>
+__device__ __forceinline__ void mend_row(const PagedDev& a, float (&o)[NC][2], int col, int step, const Tiles& t, int u0, int u1,
+                                         int seq, int h, int row, int hq, int last, int first, float m) {
+  bool bad = false;
+#pragma unroll
+  for (int c = 0; c < NC; ++c) bad = bad || !isfinite(o[c][0]) || !isfinite(o[c][1]);
+  if (!bad) return;
+  const int32_t* table = a.table + static_cast<int64_t>(seq) * a.table_st;
+  auto page_at = [&](int kv) -> int64_t {
+    const int at = kv >> a.page_log2, id = at < a.W ? __ldg(table + at) : -1;
+    return id < a.pages ? id : -1;
+  };
+  auto value = [&](int64_t page, int kv, int c) {
+    return __ldg(reinterpret_cast<const uint32_t*>(a.v_pages + page * a.vp_s0 + h * a.vp_sh +
+                                                   (kv & ((1 << a.page_log2) - 1)) * a.vp_ss + col + c * step));
+  };
+  auto sees = [&](int kv) { return kv <= last && (kv >= first || kv < a.sinks); };
+  bad = false;
+#pragma unroll 1
+  for (int u = u0; u < u1 && !bad; ++u) {
+    const int kv0 = tile_at(t, u) * TILE;
+    if (kv0 + TILE - 1 <= last && (kv0 >= first || kv0 + TILE - 1 < a.sinks)) continue;
+#pragma unroll 1
+    for (int kv = kv0; kv < kv0 + TILE && !bad; ++kv) {
+      if (sees(kv) || kv > t.lmax || (kv < t.lmin && kv >= a.sinks)) continue;
+      const int64_t page = page_at(kv);
+#pragma unroll 1
+      for (int c = 0; c < NC && page >= 0; ++c) {
+        const uint32_t w = value(page, kv, c);
+        bad = bad || !isfinite(to_float<F16>(w & 0xFFFFu)) || !isfinite(to_float<F16>(w >> 16));
+      }
+    }
+  }
+  if (!bad) return;
+#pragma unroll
+  for (int c = 0; c < NC; ++c) o[c][0] = o[c][1] = 0.0f;
+  const uint32_t* q = reinterpret_cast<const uint32_t*>(a.q + static_cast<int64_t>(row) * a.q_st + static_cast<int64_t>(hq) * a.q_sh);
+#pragma unroll 1
+  for (int u = u0; u < u1; ++u) {
+    const int kv0 = tile_at(t, u) * TILE;
+#pragma unroll 1
+    for (int kv = kv0; kv < kv0 + TILE; ++kv) {
+      const int64_t page = sees(kv) ? page_at(kv) : -1;
+      if (page < 0) continue;  // (a page outside the pool reads zeros: it adds nothing)
+      const uint32_t* k = reinterpret_cast<const uint32_t*>(a.k_pages + page * a.kp_s0 + h * a.kp_sh +
+                                                            (kv & ((1 << a.page_log2) - 1)) * a.kp_ss);
+      float s = 0.0f;
+#pragma unroll 1
+      for (int d = 0; d < D / 2; ++d) {
+        const uint32_t x = __ldg(q + d), y = __ldg(k + d);
+        s = fmaf(to_float<F16>(x & 0xFFFFu), to_float<F16>(y & 0xFFFFu), s);
+        s = fmaf(to_float<F16>(x >> 16), to_float<F16>(y >> 16), s);
+      }
+      const float p = ex2(fmaf(s, a.scale_log2, -m));
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        const uint32_t w = value(page, kv, c);
+        o[c][0] = fmaf(p, to_float<F16>(w & 0xFFFFu), o[c][0]);
+        o[c][1] = fmaf(p, to_float<F16>(w >> 16), o[c][1]);
+      }
+    }
+  }
+}
 
 // ============================================================ few rows: split over keys
 constexpr int kSplitTile = 64;
@@ -590,6 +666,9 @@ __global__ void __launch_bounds__(SplitShape<D, MT, TEAMS>::kThreads, SplitShape
               const float2 e = *reinterpret_cast<const float2*>(src + k * MT * 8 * Sh::kMergePitch + n * 8);
               v[n][0] += e.x, v[n][1] += e.y;
             }
+          if (r < rows && w.s.n > 1)  // (one token: no row sees what another does not)
+            mend_row<D, F16, kSplitTile, D / 8>(a, v, c2, 8, w.t, w.at, w.at + count, w.i, w.h, w.s.q0 + r / a.G,
+                                                w.h * a.G + r % a.G, lim[x], low[x], top);
           if (r < rows && whole) {
 #pragma unroll
             for (int n = 0; n < D / 8; ++n) *reinterpret_cast<uint32_t*>(dst + n * 8) = pack16<F16>(v[n][0] * inv, v[n][1] * inv);
@@ -1255,6 +1334,23 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           __syncwarp();
           if (lane == 0) mbar_arrive(&o_empty[g]);
         }
+        bool finite = true;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) finite = finite && isfinite(__uint_as_float(o[i]));
+        if (!finite && stored && work > 0) {
+          // (the segment's tiles, counted as tile_at counts them)
+          Tiles tl;
+          tl.lmin = sg->lmin, tl.lmax = sg->lmax, tl.t0 = sg->main0 / kTileN, tl.main = 1;
+          tl.sink = sg->sink_end > 0 ? sg->sink_end / kTileN : 0;
+          const int k0 = sg->kv0 / kTileN, u0 = k0 < tl.sink ? k0 : k0 - tl.t0 + tl.sink;
+          float f[16][2];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) f[i >> 1][i & 1] = __uint_as_float(o[i]);
+          mend_row<D, F16, kTileN, 16>(a, f, kHalfO * hc + c * 32, 2, tl, u0, u0 + sg->n, sg->i, sg->h, sg->q0 + sg->tok0 + tok,
+                                       sg->h * a.G + r % a.G, my_last, my_first, m_run);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(f[i >> 1][i & 1]);
+        }
         if (stored && whole) {
 #pragma unroll
           for (int i = 0; i < 32; i += 8) {
@@ -1593,6 +1689,8 @@ extern "C" int qik_paged_attention(const qik_paged_attn_args* args, void* ws, si
   d.out = static_cast<uint16_t*>(A.out);
   d.table = A.page_table, d.lens = A.seq_lens, d.starts = A.query_starts;
   d.status = status;
+  d.k_pages = static_cast<const uint16_t*>(A.k_pages), d.v_pages = static_cast<const uint16_t*>(A.v_pages);
+  d.kp_s0 = A.kp_s0, d.kp_sh = A.kp_sh, d.kp_ss = A.kp_ss, d.vp_s0 = A.vp_s0, d.vp_sh = A.vp_sh, d.vp_ss = A.vp_ss;
   d.q_st = A.q_st, d.q_sh = A.q_sh, d.o_st = A.o_st, d.o_sh = A.o_sh, d.table_st = A.table_st;
   d.B = static_cast<int>(A.B), d.T = static_cast<int>(A.T), d.HK = static_cast<int>(A.HK);
   d.G = static_cast<int>(A.HQ / A.HK), d.W = static_cast<int>(A.W), d.pages = static_cast<int>(A.pages);

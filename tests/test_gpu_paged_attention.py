@@ -246,3 +246,39 @@ def test_empty_calls():
     out = paged_attention(q, k, k, torch.zeros(2, 0, **i32), torch.zeros(2, **i32), torch.tensor([0, 1, 2], **i32), 1)
     torch.cuda.synchronize()
     assert (out == 0).all()
+
+
+@pytest.mark.parametrize("dtype,dim", [(torch.bfloat16, 128), (torch.float16, 64)])
+@pytest.mark.parametrize("new,kv,window", [([9, 1, 4], [200, 64, 1000], 0), ([5], [700], 30), ([13], [40], 0), ([60], [130], 20),
+                                           ([200, 90], [200, 700], 0), ([300], [900], 64), ([129, 7], [2000, 9], 0)])
+def test_infinities_in_keys_that_some_rows_see(new, kv, window, dtype, dim):
+    """V with infinities and NaN at new tokens and at a window's edge: rows that do not see the
+    token are exact, rows that do have what the formula gives in each column."""
+    s = make(new, kv, 8, 2, dim, 32, dtype, seed=17)
+    odd = []
+    for i, (n, m) in enumerate(zip(new, kv)):
+        for back, value, col in ((0, float("nan"), 3), (n // 2, float("inf"), 7), (n - 1, -float("inf"), dim - 1),
+                                 (min(m - 1, window + n // 3), float("inf"), 20)):
+            t = m - 1 - back
+            s["v_pages"][s["page_table"][i, t // 32].long(), 1, t % 32, col] = value
+            odd.append((i, t, col))
+    got = run(s, window=window)
+    finite = dict(s, v_pages=torch.where(s["v_pages"].isfinite(), s["v_pages"], torch.zeros_like(s["v_pages"])))
+    want, mass = exact(finite, new, kv, window=window)
+    starts = [0]
+    for n in new:
+        starts.append(starts[-1] + n)
+    touched = torch.zeros(got.shape, dtype=torch.bool, device=DEV)
+    for i, t, col in set(odd):
+        value = s["v_pages"][s["page_table"][i, t // 32].long(), 1, t % 32, col].double()
+        for j in range(new[i]):
+            last = kv[i] - new[i] + j
+            if t <= last and (not window or t > last - window):
+                want[starts[i] + j, 4:, col] += value  # p is positive
+                touched[starts[i] + j, 4:, col] = True
+    assert torch.equal(got.isnan(), want.isnan())
+    assert torch.equal(got.isinf(), want.isinf()) and torch.equal(got[got.isinf()].double(), want[want.isinf()])
+    half = torch.finfo(dtype).eps / 2
+    bound = (half + 1.5e-4) * mass + half * want.abs() + (max(kv) * 2.0 ** -22 if dtype == torch.float16 else 0) + 1e-6
+    assert ((got.double() - want).abs()[~touched] <= bound[~touched]).all()
+    assert touched.any() and not touched.all()
