@@ -58,7 +58,7 @@ struct PagedDev {
   float scale_log2;
   bool causal, unit_mode;
   int tile_tok;          // tile kernel: tokens of a 128-row query tile (128 / G)
-  int lo_rows, hi_rows;  // rows (new tokens x group) of the sequences this launch takes
+  int hi_rows;           // split kernel: most rows (new tokens x group) of a sequence
 };
 
 struct Seq {
@@ -255,7 +255,7 @@ __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
 __device__ __forceinline__ int split_tiles(const PagedDev& a, int i, Seq& s, Tiles& t) {
   s = seq_of(a, i);
   const int rows = s.n * a.G;
-  if (rows <= a.lo_rows || rows > a.hi_rows) return 0;
+  if (rows == 0 || rows > a.hi_rows) return 0;
   t = tiles_of<kSplitTile>(a, s, 0, s.n);
   return max(1, t.sink + t.main);
 }
@@ -730,8 +730,7 @@ struct Block {
   int left;              // work left in the CTA's range, this unit's not counted
 };
 __device__ __forceinline__ int row_blocks(const PagedDev& a, const Seq& s) {
-  const int rows = s.n * a.G;
-  return rows > a.lo_rows ? (s.n + 2 * a.tile_tok - 1) / (2 * a.tile_tok) : 0;
+  return (s.n + 2 * a.tile_tok - 1) / (2 * a.tile_tok);
 }
 __device__ __forceinline__ Tiles block_tiles(const PagedDev& a, const Seq& s, int rb) {
   const int j0 = rb * 2 * a.tile_tok;
@@ -739,6 +738,7 @@ __device__ __forceinline__ Tiles block_tiles(const PagedDev& a, const Seq& s, in
 }
 // (a unit whose rows see no key still has one tile, so that its rows are written as zeros)
 __device__ __forceinline__ int block_work(const PagedDev& a, const Seq& s, int rb) {
+  if (a.unit_mode) return 1;  // (one CTA a unit)
   const Tiles t = block_tiles(a, s, rb);
   return max(1, t.sink + t.main) + kUnitCost;
 }
@@ -820,7 +820,7 @@ __device__ __forceinline__ bool open_range(const PagedDev& a, Block& b, int& sha
     sum += mine;
   }
   int total, excl = scan_block(sum, total);
-  share = max(a.min_share, static_cast<int>((static_cast<uint32_t>(total) + gridDim.x - 1) / gridDim.x));
+  share = a.unit_mode ? 1 : max(a.min_share, static_cast<int>((static_cast<uint32_t>(total) + gridDim.x - 1) / gridDim.x));
   const long long begin = static_cast<long long>(share) * blockIdx.x;
   if (begin >= total) return false;
   const int want = static_cast<int>(begin);
@@ -868,7 +868,13 @@ __device__ __forceinline__ bool open_range(const PagedDev& a, Block& b, int& sha
       break;
     }
   }
-  return open_block(a, b, rest);  // (uniform: the range may end before the unit's first tile)
+  if (a.unit_mode) {
+    rest = 0;
+    b.left = 0x3FFFFFFF;
+  }
+  const bool any = open_block(a, b, rest);
+  if (a.unit_mode) b.left = 0;
+  return any;  // (uniform: the range may end before the unit's first tile)
 }
 
 // 32 of the D / 2 columns of O that each of a row's two threads has.
@@ -989,7 +995,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   Block b;
   int share;
   const bool any = open_range(a, b, share, slot);
-  if (threadIdx.x == 0) a.ws_desc[blockIdx.x] = make_int4(-1, 0, 0, 0);
+  if (threadIdx.x == 0 && !a.unit_mode) a.ws_desc[blockIdx.x] = make_int4(-1, 0, 0, 0);
   if (!any) {
     pdl_trigger();
     return;
@@ -1392,44 +1398,36 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 constexpr int kJoinRows = 2;
 constexpr int kJoinWarps = 2;
 
-struct JoinSet {  // one kernel's pieces
-  const float* o;
-  const float2* ml;
-  const int4* desc;
-  int ctas, rows, blocks;  // its CTAs, rows of a piece, join CTAs for each of its CTAs
-};
 struct JoinDev {
   uint16_t* out;
   int64_t o_st, o_sh;
-  int G, tile_tok;
-  JoinSet split, tile;
+  const float* ws_o;
+  const float2* ws_ml;
+  const int4* ws_desc;
+  int G, tile_tok, slot_rows;
+  bool toks;  // the unit's rows are counted in query tiles of 128 (tile kernel)
 };
+// blockIdx.x: the kernel's CTAs; blockIdx.y: rows of the unit.
 template <int D, bool F16>
 __global__ void __launch_bounds__(kJoinWarps * 32, 16) paged_join_kernel(const JoinDev a) {
   using Vec = typename std::conditional<D == 128, float4, float2>::type;
-  // the tile kernel's units first (they are the larger)
-  const int lane = threadIdx.x & 31, tile_blocks = a.tile.ctas * a.tile.blocks;
-  const bool toks = static_cast<int>(blockIdx.x) < tile_blocks;  // rows counted in query tiles of 128
-  const int block = toks ? blockIdx.x : blockIdx.x - tile_blocks, blocks = toks ? a.tile.blocks : a.split.blocks;
-  const float* ws_o = toks ? a.tile.o : a.split.o;
-  const float2* ws_ml = toks ? a.tile.ml : a.split.ml;
-  const int slot_rows = toks ? a.tile.rows : a.split.rows;
-  const int cta = block / blocks, r0 = (block % blocks * kJoinWarps + (threadIdx.x >> 5)) * kJoinRows;
+  const int lane = threadIdx.x & 31, cta = blockIdx.x;
+  const int r0 = (blockIdx.y * kJoinWarps + (threadIdx.x >> 5)) * kJoinRows;
   pdl_wait();
-  const int4 d = __ldcg((toks ? a.tile.desc : a.split.desc) + cta);  // first row of q, head, further pieces, rows (tokens)
+  const int4 d = __ldcg(a.ws_desc + cta);  // first row of q, head, further pieces, rows (tokens)
   uint16_t* dst[kJoinRows];
   bool any = false;
 #pragma unroll
   for (int k = 0; k < kJoinRows; ++k) {
     const int r = r0 + k;
-    const int in = toks ? r % kTileM : r, tok = toks ? in / a.G + r / kTileM * a.tile_tok : r / a.G;
-    const bool mine = d.x >= 0 && (toks ? in < a.tile_tok * a.G && tok < d.w : r < d.w);
+    const int in = a.toks ? r % kTileM : r, tok = a.toks ? in / a.G + r / kTileM * a.tile_tok : r / a.G;
+    const bool mine = d.x >= 0 && (a.toks ? in < a.tile_tok * a.G && tok < d.w : r < d.w);
     any = any || mine;
     dst[k] = mine ? a.out + static_cast<int64_t>(d.x + tok) * a.o_st + static_cast<int64_t>(d.y * a.G + in % a.G) * a.o_sh : nullptr;
   }
   if (any) {
     const int pieces = 1 + d.z;
-    auto at = [&](int p, int k) { return static_cast<int64_t>(p == 0 ? 2 * cta + 1 : 2 * (cta + p)) * slot_rows + r0 + k; };
+    auto at = [&](int p, int k) { return static_cast<int64_t>(p == 0 ? 2 * cta + 1 : 2 * (cta + p)) * a.slot_rows + r0 + k; };
     float2 ml[2][kJoinRows];
     Vec v[2][kJoinRows];
     float top[kJoinRows], sum[kJoinRows], acc[kJoinRows][D / 32];
@@ -1437,14 +1435,14 @@ __global__ void __launch_bounds__(kJoinWarps * 32, 16) paged_join_kernel(const J
     for (int p = 0; p < 2; ++p)
 #pragma unroll
       for (int k = 0; k < kJoinRows; ++k) {
-        ml[p][k] = __ldcg(ws_ml + at(p, k));
-        v[p][k] = __ldcg(reinterpret_cast<const Vec*>(ws_o + at(p, k) * D) + lane);
+        ml[p][k] = __ldcg(a.ws_ml + at(p, k));
+        v[p][k] = __ldcg(reinterpret_cast<const Vec*>(a.ws_o + at(p, k) * D) + lane);
       }
 #pragma unroll
     for (int k = 0; k < kJoinRows; ++k) {
       top[k] = fmaxf(ml[0][k].x, ml[1][k].x);
       if (pieces > 2) {
-        for (int p = 2 + lane; p < pieces; p += 32) top[k] = fmaxf(top[k], __ldcg(ws_ml + at(p, k)).x);
+        for (int p = 2 + lane; p < pieces; p += 32) top[k] = fmaxf(top[k], __ldcg(a.ws_ml + at(p, k)).x);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], o));
       }
@@ -1469,8 +1467,8 @@ __global__ void __launch_bounds__(kJoinWarps * 32, 16) paged_join_kernel(const J
 #pragma unroll
         for (int k = 0; k < kJoinRows; ++k)
           if (p0 + p < pieces) {
-            ml[p][k] = __ldcg(ws_ml + at(p0 + p, k));
-            v[p][k] = __ldcg(reinterpret_cast<const Vec*>(ws_o + at(p0 + p, k) * D) + lane);
+            ml[p][k] = __ldcg(a.ws_ml + at(p0 + p, k));
+            v[p][k] = __ldcg(reinterpret_cast<const Vec*>(a.ws_o + at(p0 + p, k) * D) + lane);
           }
 #pragma unroll
       for (int p = 0; p < 2; ++p)
@@ -1496,44 +1494,48 @@ __global__ void __launch_bounds__(kJoinWarps * 32, 16) paged_join_kernel(const J
 constexpr int kSplitRows = 64;  // most rows of a sequence that the split kernel takes
 
 struct PagedPlan {
-  bool split, tile, unit_mode;
-  int split_mt, split_ctas, tile_ctas;
-  size_t split_o, split_ml, split_desc, tile_o, tile_ml, tile_desc, bytes;  // workspace offsets
+  bool split;      // the split kernel, else the tile kernel
+  bool unit_mode;  // one CTA a unit, nothing to join
+  int mt, ctas, slot_rows;
+  size_t o, ml, desc, bytes;  // workspace offsets
 };
 
+// Up to kSplitRows rows in every sequence: the split kernel; else the tile kernel for all of them (a
+// single token among chunks still loads its keys at three quarters of the HBM rate there, and
+// one kernel and its join are launched instead of two).  Short contexts (8 tiles of the kernel's
+// size) with units for at most two CTAs an SM are not cut: a join costs more than it gives.
 static PagedPlan paged_plan(const qik_paged_attn_args& A) {
   PagedPlan p = {};
   const int64_t G = A.HQ / A.HK, max_rows = A.max_new * G;
   const int sms = sm_count();
-  // sequences of at most kSplitRows rows may exist unless all have max_new tokens
-  p.tile = max_rows > kSplitRows;
-  p.split = !p.tile || A.T != A.B * A.max_new;
-  size_t at = 0;
+  p.split = max_rows <= kSplitRows;
+  int64_t units;
+  if (p.split) {
+    p.mt = max_rows <= 16 ? 1 : max_rows <= 32 ? 2 : 4;
+    units = A.B * A.HK;
+    p.unit_mode = A.max_kv <= 8 * kSplitTile;
+    p.ctas = sms * (p.mt == 1 ? 2 : 1);
+    p.slot_rows = p.mt * 16;
+  } else {
+    const int64_t block = 2 * (kTileM / G), by_rows = A.T / block + A.B, by_seq = A.B * ((A.max_new + block - 1) / block);
+    units = (by_rows < by_seq ? by_rows : by_seq) * A.HK;
+    p.unit_mode = A.max_kv <= 8 * kTileN && units <= 2 * sms;
+    p.ctas = sms;
+    p.slot_rows = kTileRows;
+  }
+  if (p.unit_mode) {
+    p.ctas = static_cast<int>(units);
+    return p;
+  }
   auto take = [&](size_t bytes) {
-    const size_t here = at;
-    at += (bytes + 255) / 256 * 256;
+    const size_t here = p.bytes;
+    p.bytes += (bytes + 255) / 256 * 256;
     return here;
   };
-  if (p.split) {
-    p.split_mt = max_rows <= 16 ? 1 : max_rows <= 32 ? 2 : 4;
-    // short contexts (at most 8 tiles): one CTA for each (sequence, head), nothing to join
-    p.unit_mode = A.max_kv <= 8 * kSplitTile;
-    p.split_ctas = p.unit_mode ? static_cast<int>(A.B * A.HK) : sms * (p.split_mt == 1 ? 2 : 1);
-    if (!p.unit_mode) {
-      const size_t rows = static_cast<size_t>(2) * p.split_ctas * p.split_mt * 16;
-      p.split_o = take(rows * A.D * sizeof(float));
-      p.split_ml = take(rows * sizeof(float2));
-      p.split_desc = take(p.split_ctas * sizeof(int4));
-    }
-  }
-  if (p.tile) {
-    p.tile_ctas = sms;
-    const size_t rows = static_cast<size_t>(2) * sms * kTileRows;
-    p.tile_o = take(rows * A.D * sizeof(float));
-    p.tile_ml = take(rows * sizeof(float2));
-    p.tile_desc = take(sms * sizeof(int4));
-  }
-  p.bytes = at;
+  const size_t rows = static_cast<size_t>(2) * p.ctas * p.slot_rows;
+  p.o = take(rows * A.D * sizeof(float));
+  p.ml = take(rows * sizeof(float2));
+  p.desc = take(p.ctas * sizeof(int4));
   return p;
 }
 
@@ -1595,50 +1597,29 @@ static cudaError_t launch_split(const CUtensorMap& tk, const CUtensorMap& tv, co
   return launch_kernel(paged_split_kernel<D, MT, TEAMS, F16>, dim3(ctas), dim3(Sh::kThreads), Sh::kBytes, st, true, tk, tv, d);
 }
 template <int D, bool F16>
-static cudaError_t launch_paged(const qik_paged_attn_args& A, const PagedPlan& p, PagedDev d, uint8_t* ws,
-                                const CUtensorMap* maps, cudaStream_t st) {
-  cudaError_t e = cudaSuccess;
+static cudaError_t launch_paged(const PagedPlan& p, PagedDev d, const CUtensorMap* maps, cudaStream_t st) {
+  cudaError_t e;
   if (p.split) {
-    PagedDev s = d;
-    s.lo_rows = 0;
-    s.hi_rows = p.split_mt * 16;
-    s.unit_mode = p.unit_mode;
-    s.ws_o = reinterpret_cast<float*>(ws + p.split_o);
-    s.ws_ml = reinterpret_cast<float2*>(ws + p.split_ml);
-    s.ws_desc = reinterpret_cast<int4*>(ws + p.split_desc);
-    const bool few = p.unit_mode && p.split_ctas <= sm_count();
-    e = p.split_mt == 1   ? (few ? launch_split<D, 1, 2, F16>(maps[0], maps[1], s, p.split_ctas, st)
-                                 : launch_split<D, 1, 1, F16>(maps[0], maps[1], s, p.split_ctas, st))
-        : p.split_mt == 2 ? launch_split<D, 2, 1, F16>(maps[0], maps[1], s, p.split_ctas, st)
-                          : launch_split<D, 4, 1, F16>(maps[0], maps[1], s, p.split_ctas, st);
-    if (e != cudaSuccess) return e;
-  }
-  if (p.tile) {
+    const bool few = p.unit_mode && p.ctas <= sm_count();
+    d.hi_rows = p.slot_rows;
+    d.min_share = 4;
+    e = p.mt == 1   ? (few ? launch_split<D, 1, 2, F16>(maps[0], maps[1], d, p.ctas, st)
+                           : launch_split<D, 1, 1, F16>(maps[0], maps[1], d, p.ctas, st))
+        : p.mt == 2 ? launch_split<D, 2, 1, F16>(maps[0], maps[1], d, p.ctas, st)
+                    : launch_split<D, 4, 1, F16>(maps[0], maps[1], d, p.ctas, st);
+  } else {
     using Sh = TileShape<D>;
     static std::once_flag once[64];
     e = allow_smem(paged_tile_kernel<D, F16>, Sh::kBytes, once);
     if (e != cudaSuccess) return e;
-    d.lo_rows = kSplitRows;
-    d.hi_rows = 0x7FFFFFFF;
-    d.ws_o = reinterpret_cast<float*>(ws + p.tile_o);
-    d.ws_ml = reinterpret_cast<float2*>(ws + p.tile_ml);
-    d.ws_desc = reinterpret_cast<int4*>(ws + p.tile_desc);
-    e = launch_kernel(paged_tile_kernel<D, F16>, dim3(p.tile_ctas), dim3(kTileThreads), Sh::kBytes, st, true, maps[2], maps[3],
-                      maps[4], d);
-    if (e != cudaSuccess) return e;
+    d.min_share = kUnitCost + 5;
+    e = launch_kernel(paged_tile_kernel<D, F16>, dim3(p.ctas), dim3(kTileThreads), Sh::kBytes, st, true, maps[0], maps[1],
+                      maps[2], d);
   }
-  // one join for both kernels' pieces
-  JoinDev j = {d.out, d.o_st, d.o_sh, d.G, d.tile_tok, {}, {}};
-  const auto set = [&](size_t o, size_t ml, size_t desc, int ctas, int rows) {
-    return JoinSet{reinterpret_cast<const float*>(ws + o), reinterpret_cast<const float2*>(ws + ml),
-                   reinterpret_cast<const int4*>(ws + desc), ctas, rows, rows / (kJoinRows * kJoinWarps)};
-  };
-  if (p.split && !p.unit_mode) j.split = set(p.split_o, p.split_ml, p.split_desc, p.split_ctas, p.split_mt * 16);
-  if (p.tile) j.tile = set(p.tile_o, p.tile_ml, p.tile_desc, p.tile_ctas, kTileRows);
-  const int blocks = j.split.ctas * j.split.blocks + j.tile.ctas * j.tile.blocks;
-  if (blocks > 0)
-    e = launch_kernel(paged_join_kernel<D, F16>, dim3(blocks), dim3(kJoinWarps * 32), 0, st, true, j);
-  return e;
+  if (e != cudaSuccess || p.unit_mode) return e;
+  const JoinDev j = {d.out, d.o_st, d.o_sh, d.ws_o, d.ws_ml, d.ws_desc, d.G, d.tile_tok, p.slot_rows, !p.split};
+  return launch_kernel(paged_join_kernel<D, F16>, dim3(p.ctas, p.slot_rows / (kJoinRows * kJoinWarps)), dim3(kJoinWarps * 32), 0,
+                       st, true, j);
 }
 
 }  // namespace qik
@@ -1667,21 +1648,17 @@ extern "C" int qik_paged_attention(const qik_paged_attn_args* args, void* ws, si
   QIK_REQUIRE(p.bytes == 0 || (ws && ws_bytes >= p.bytes), "qik_paged_attention: workspace of %zu bytes, %zu needed",
               ws_bytes, p.bytes);
   const bool f16 = (A.flags & QIK_PAGED_F16) != 0;
-  CUtensorMap maps[5];
-  if (p.split) {
-    rc = page_map(&maps[0], A.k_pages, f16, A, A.kp_s0, A.kp_sh, A.kp_ss, kSplitTile, static_cast<uint32_t>(A.D / 64));
-    if (!rc) rc = page_map(&maps[1], A.v_pages, f16, A, A.vp_s0, A.vp_sh, A.vp_ss, kSplitTile, static_cast<uint32_t>(A.D / 64));
-  }
-  if (!rc && p.tile) {
-    rc = page_map(&maps[2], A.k_pages, f16, A, A.kp_s0, A.kp_sh, A.kp_ss, kTileN, 1);
-    if (!rc) rc = page_map(&maps[3], A.v_pages, f16, A, A.vp_s0, A.vp_sh, A.vp_ss, kTileN, 1);
-    if (!rc) {  // q: (64 columns, head, token, half), boxes of a group's heads and a query tile's tokens
-      const uint64_t dims[4] = {64, static_cast<uint64_t>(A.HQ), static_cast<uint64_t>(A.T), static_cast<uint64_t>(A.D / 64)};
-      const uint64_t strides[3] = {static_cast<uint64_t>(A.q_sh * 2), static_cast<uint64_t>(A.q_st * 2), 128};
-      const uint32_t group = static_cast<uint32_t>(A.HQ / A.HK), box[4] = {64, group, 128 / group, 1};
-      rc = make_tmap_nd(&maps[4], A.q, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, dims,
-                        strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
-    }
+  const int64_t tile = p.split ? kSplitTile : kTileN;
+  const uint32_t halves = p.split ? static_cast<uint32_t>(A.D / 64) : 1;
+  CUtensorMap maps[3];
+  rc = page_map(&maps[0], A.k_pages, f16, A, A.kp_s0, A.kp_sh, A.kp_ss, tile, halves);
+  if (!rc) rc = page_map(&maps[1], A.v_pages, f16, A, A.vp_s0, A.vp_sh, A.vp_ss, tile, halves);
+  if (!rc && !p.split) {  // q: (64 columns, head, token, half), boxes of a group's heads and a query tile's tokens
+    const uint64_t dims[4] = {64, static_cast<uint64_t>(A.HQ), static_cast<uint64_t>(A.T), static_cast<uint64_t>(A.D / 64)};
+    const uint64_t strides[3] = {static_cast<uint64_t>(A.q_sh * 2), static_cast<uint64_t>(A.q_st * 2), 128};
+    const uint32_t group = static_cast<uint32_t>(A.HQ / A.HK), box[4] = {64, group, kTileM / group, 1};
+    rc = make_tmap_nd(&maps[2], A.q, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, dims, strides,
+                      box, CU_TENSOR_MAP_SWIZZLE_128B);
   }
   if (rc) return rc;
   PagedDev d = {};
@@ -1698,13 +1675,16 @@ extern "C" int qik_paged_attention(const qik_paged_attn_args* args, void* ws, si
   d.max_new = static_cast<int>(A.max_new);
   d.tile_tok = 128 / d.G;
   d.window = A.window, d.sinks = A.window > 0 ? A.sinks : 0;
-  d.min_share = 4;
+  d.unit_mode = p.unit_mode;
   d.scale_log2 = A.sm_scale * 1.4426950408889634f;
   d.causal = (A.flags & QIK_PAGED_CAUSAL) != 0;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   uint8_t* w = static_cast<uint8_t*>(ws);
-  cudaError_t e = A.D == 128 ? (f16 ? launch_paged<128, true>(A, p, d, w, maps, st) : launch_paged<128, false>(A, p, d, w, maps, st))
-                             : (f16 ? launch_paged<64, true>(A, p, d, w, maps, st) : launch_paged<64, false>(A, p, d, w, maps, st));
+  d.ws_o = reinterpret_cast<float*>(w + p.o);
+  d.ws_ml = reinterpret_cast<float2*>(w + p.ml);
+  d.ws_desc = reinterpret_cast<int4*>(w + p.desc);
+  cudaError_t e = A.D == 128 ? (f16 ? launch_paged<128, true>(p, d, maps, st) : launch_paged<128, false>(p, d, maps, st))
+                             : (f16 ? launch_paged<64, true>(p, d, maps, st) : launch_paged<64, false>(p, d, maps, st));
   QIK_TRY_CUDA(e);
   return check_launch("qik_paged_attention");
 }
