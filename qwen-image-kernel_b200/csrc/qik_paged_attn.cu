@@ -1496,45 +1496,61 @@ constexpr int kSplitRows = 64;  // most rows of a sequence that the split kernel
 struct PagedPlan {
   bool split;      // the split kernel, else the tile kernel
   bool unit_mode;  // one CTA a unit, nothing to join
-  int mt, ctas, slot_rows;
+  int mt, ctas, slot_rows, min_share, join_blocks;
   size_t o, ml, desc, bytes;  // workspace offsets
 };
 
 // Up to kSplitRows rows in every sequence: the split kernel; else the tile kernel for all of them (a
 // single token among chunks still loads its keys at three quarters of the HBM rate there, and
-// one kernel and its join are launched instead of two).  Short contexts (8 tiles of the kernel's
-// size) with units for at most two CTAs an SM are not cut: a join costs more than it gives.
+// one kernel and its join are launched instead of two).  Short contexts are not cut: a join costs
+// more than it gives (with units of at most 4 tiles instead of 8 left whole, the calls between
+// took twice as long).  Shares have at least 4 tiles (split: 2 and 8 measured slower) or a unit's
+// change and 2 (tile; 5 took 1% longer over 100 calls of mixed sizes, up to 23% on the small).
 static PagedPlan paged_plan(const qik_paged_attn_args& A) {
   PagedPlan p = {};
   const int64_t G = A.HQ / A.HK, max_rows = A.max_new * G;
   const int sms = sm_count();
   p.split = max_rows <= kSplitRows;
-  int64_t units;
+  // the keys that a row can see bound the tiles of a unit
+  const int64_t seen = A.window > 0 && A.window + A.max_new < A.max_kv ? A.window + A.max_new : A.max_kv;
+  const int64_t sinks = A.window > 0 ? A.sinks : 0, size = p.split ? kSplitTile : kTileN;
+  const int64_t tiles = (seen + size - 1) / size + (seen < A.max_kv ? 1 + (sinks + size - 1) / size : 0);
+  int64_t units, work, rows = 0;
   if (p.split) {
     p.mt = max_rows <= 16 ? 1 : max_rows <= 32 ? 2 : 4;
     units = A.B * A.HK;
-    p.unit_mode = A.max_kv <= 8 * kSplitTile;
+    work = units * tiles;
+    // two teams of warps (mt 1 with units for at most the SMs) take a tile in 0.35 us, one in 0.65
+    p.unit_mode = tiles <= 8 || (tiles <= 14 && (p.mt == 1 || units >= sms));
     p.ctas = sms * (p.mt == 1 ? 2 : 1);
+    p.min_share = 4;
     p.slot_rows = p.mt * 16;
+    rows = max_rows;
   } else {
     const int64_t block = 2 * (kTileM / G), by_rows = A.T / block + A.B, by_seq = A.B * ((A.max_new + block - 1) / block);
     units = (by_rows < by_seq ? by_rows : by_seq) * A.HK;
-    p.unit_mode = A.max_kv <= 8 * kTileN && units <= 2 * sms;
+    work = units * (tiles + kUnitCost);
+    p.unit_mode = tiles <= 8 && units <= 2 * sms;
     p.ctas = sms;
+    p.min_share = kUnitCost + 2;
     p.slot_rows = kTileRows;
+    rows = A.max_new <= block / 2 ? kTileM : kTileRows;
   }
   if (p.unit_mode) {
     p.ctas = static_cast<int>(units);
     return p;
   }
+  // no more CTAs than there can be shares
+  if ((work + p.min_share - 1) / p.min_share < p.ctas) p.ctas = static_cast<int>((work + p.min_share - 1) / p.min_share);
+  p.join_blocks = static_cast<int>((rows + kJoinRows * kJoinWarps - 1) / (kJoinRows * kJoinWarps));
   auto take = [&](size_t bytes) {
     const size_t here = p.bytes;
     p.bytes += (bytes + 255) / 256 * 256;
     return here;
   };
-  const size_t rows = static_cast<size_t>(2) * p.ctas * p.slot_rows;
-  p.o = take(rows * A.D * sizeof(float));
-  p.ml = take(rows * sizeof(float2));
+  const size_t slots = static_cast<size_t>(2) * p.ctas * p.slot_rows;
+  p.o = take(slots * A.D * sizeof(float));
+  p.ml = take(slots * sizeof(float2));
   p.desc = take(p.ctas * sizeof(int4));
   return p;
 }
@@ -1602,7 +1618,6 @@ static cudaError_t launch_paged(const PagedPlan& p, PagedDev d, const CUtensorMa
   if (p.split) {
     const bool few = p.unit_mode && p.ctas <= sm_count();
     d.hi_rows = p.slot_rows;
-    d.min_share = 4;
     e = p.mt == 1   ? (few ? launch_split<D, 1, 2, F16>(maps[0], maps[1], d, p.ctas, st)
                            : launch_split<D, 1, 1, F16>(maps[0], maps[1], d, p.ctas, st))
         : p.mt == 2 ? launch_split<D, 2, 1, F16>(maps[0], maps[1], d, p.ctas, st)
@@ -1612,13 +1627,12 @@ static cudaError_t launch_paged(const PagedPlan& p, PagedDev d, const CUtensorMa
     static std::once_flag once[64];
     e = allow_smem(paged_tile_kernel<D, F16>, Sh::kBytes, once);
     if (e != cudaSuccess) return e;
-    d.min_share = kUnitCost + 5;
     e = launch_kernel(paged_tile_kernel<D, F16>, dim3(p.ctas), dim3(kTileThreads), Sh::kBytes, st, true, maps[0], maps[1],
                       maps[2], d);
   }
   if (e != cudaSuccess || p.unit_mode) return e;
   const JoinDev j = {d.out, d.o_st, d.o_sh, d.ws_o, d.ws_ml, d.ws_desc, d.G, d.tile_tok, p.slot_rows, !p.split};
-  return launch_kernel(paged_join_kernel<D, F16>, dim3(p.ctas, p.slot_rows / (kJoinRows * kJoinWarps)), dim3(kJoinWarps * 32), 0,
+  return launch_kernel(paged_join_kernel<D, F16>, dim3(p.ctas, p.join_blocks), dim3(kJoinWarps * 32), 0,
                        st, true, j);
 }
 
@@ -1675,7 +1689,7 @@ extern "C" int qik_paged_attention(const qik_paged_attn_args* args, void* ws, si
   d.max_new = static_cast<int>(A.max_new);
   d.tile_tok = 128 / d.G;
   d.window = A.window, d.sinks = A.window > 0 ? A.sinks : 0;
-  d.unit_mode = p.unit_mode;
+  d.unit_mode = p.unit_mode, d.min_share = p.min_share;
   d.scale_log2 = A.sm_scale * 1.4426950408889634f;
   d.causal = (A.flags & QIK_PAGED_CAUSAL) != 0;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
