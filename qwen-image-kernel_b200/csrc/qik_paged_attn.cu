@@ -1409,7 +1409,7 @@ struct JoinDev {
 };
 // blockIdx.x: the kernel's CTAs; blockIdx.y: rows of the unit.
 template <int D, bool F16>
-__global__ void __launch_bounds__(kJoinWarps * 32, 16) paged_join_kernel(const JoinDev a) {
+__global__ void __launch_bounds__(kJoinWarps * 32, 12) paged_join_kernel(const JoinDev a) {
   using Vec = typename std::conditional<D == 128, float4, float2>::type;
   const int lane = threadIdx.x & 31, cta = blockIdx.x;
   const int r0 = (blockIdx.y * kJoinWarps + (threadIdx.x >> 5)) * kJoinRows;
@@ -1461,20 +1461,22 @@ __global__ void __launch_bounds__(kJoinWarps * 32, 16) paged_join_kernel(const J
     for (int p = 0; p < 2; ++p)
 #pragma unroll
       for (int k = 0; k < kJoinRows; ++k) add(k, ml[p][k], v[p][k]);
-    for (int p0 = 2; p0 < pieces; p0 += 2) {
+    for (int p0 = 2; p0 < pieces; p0 += 4) {  // (one long sequence: dozens of pieces)
+      float2 more_ml[4][kJoinRows];
+      Vec more_v[4][kJoinRows];
 #pragma unroll
-      for (int p = 0; p < 2; ++p)
+      for (int p = 0; p < 4; ++p)
 #pragma unroll
         for (int k = 0; k < kJoinRows; ++k)
           if (p0 + p < pieces) {
-            ml[p][k] = __ldcg(a.ws_ml + at(p0 + p, k));
-            v[p][k] = __ldcg(reinterpret_cast<const Vec*>(a.ws_o + at(p0 + p, k) * D) + lane);
+            more_ml[p][k] = __ldcg(a.ws_ml + at(p0 + p, k));
+            more_v[p][k] = __ldcg(reinterpret_cast<const Vec*>(a.ws_o + at(p0 + p, k) * D) + lane);
           }
 #pragma unroll
-      for (int p = 0; p < 2; ++p)
+      for (int p = 0; p < 4; ++p)
 #pragma unroll
         for (int k = 0; k < kJoinRows; ++k)
-          if (p0 + p < pieces) add(k, ml[p][k], v[p][k]);
+          if (p0 + p < pieces) add(k, more_ml[p][k], more_v[p][k]);
     }
 #pragma unroll
     for (int k = 0; k < kJoinRows; ++k) {
