@@ -697,6 +697,9 @@ constexpr int kTileThreads = 128 + 64 * kTileSoftmaxWarps;
 constexpr float kTileRescale = 8.0f;           // O is rescaled when a maximum grows by > 2^8
 constexpr int kTilePolyFrom = 23;              // pairs of a half row from here on take 2^x on the FMA pipe
 
+__device__ __forceinline__ uint32_t bits_below(int n) {  // the lowest n bits, n clamped to [0, 32]
+  return n >= 32 ? 0xFFFFFFFFu : n <= 0 ? 0u : (1u << n) - 1u;
+}
 __device__ __forceinline__ float fmax3_nan(float a, float b, float c) {  // NaN if any is
   float d;
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
@@ -738,7 +741,6 @@ __device__ __forceinline__ Tiles block_tiles(const PagedDev& a, const Seq& s, in
 }
 // (a unit whose rows see no key still has one tile, so that its rows are written as zeros)
 __device__ __forceinline__ int block_work(const PagedDev& a, const Seq& s, int rb) {
-  if (a.unit_mode) return 1;  // (one CTA a unit)
   const Tiles t = block_tiles(a, s, rb);
   return max(1, t.sink + t.main) + kUnitCost;
 }
@@ -792,6 +794,20 @@ __device__ __forceinline__ bool next_block(const PagedDev& a, Block& b) {
 __device__ __forceinline__ bool open_range(const PagedDev& a, Block& b, int& share, int* slot) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
   Seq s;
+  if (a.unit_mode) {  // blockIdx.x: (sequence, block, head), the blocks of max_new tokens counted for all
+    const int most = (a.max_new + 2 * a.tile_tok - 1) / (2 * a.tile_tok);
+    b.h = blockIdx.x % a.HK;
+    b.rb = blockIdx.x / a.HK % most;
+    b.i = blockIdx.x / (a.HK * most);
+    b.s = seq_of(a, b.i);
+    b.blocks = row_blocks(a, b.s);
+    if (b.rb >= b.blocks) return false;
+    share = 1;
+    b.left = 0x3FFFFFFF;
+    open_block(a, b, 0);
+    b.left = 0;
+    return true;
+  }
   int blocks, mine = 0, sum = 0;
   auto look = [&](int i) {
     s = seq_of(a, min(i, a.B - 1));
@@ -808,19 +824,22 @@ __device__ __forceinline__ bool open_range(const PagedDev& a, Block& b, int& sha
     __syncthreads();
     if (lane == 31) slot[4 + warp] = incl;
     __syncthreads();
-    total = 0;
-    for (int k = 0; k < warps; ++k) {
-      if (k == warp) incl += total;
-      total += slot[4 + k];
+    int before = lane < warps ? slot[4 + lane] : 0;  // (a scan of the warps' sums by every warp)
+    const int own = before;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, before, o);
+      if (lane >= o) before += up;
     }
-    return incl - v;
+    total = __shfl_sync(0xffffffffu, before, 31);
+    return incl - v + __shfl_sync(0xffffffffu, before - own, warp);
   };
   for (int i0 = 0; i0 < a.B; i0 += blockDim.x) {
     look(i0 + threadIdx.x);
     sum += mine;
   }
   int total, excl = scan_block(sum, total);
-  share = a.unit_mode ? 1 : max(a.min_share, static_cast<int>((static_cast<uint32_t>(total) + gridDim.x - 1) / gridDim.x));
+  share = max(a.min_share, static_cast<int>((static_cast<uint32_t>(total) + gridDim.x - 1) / gridDim.x));
   const long long begin = static_cast<long long>(share) * blockIdx.x;
   if (begin >= total) return false;
   const int want = static_cast<int>(begin);
@@ -868,13 +887,7 @@ __device__ __forceinline__ bool open_range(const PagedDev& a, Block& b, int& sha
       break;
     }
   }
-  if (a.unit_mode) {
-    rest = 0;
-    b.left = 0x3FFFFFFF;
-  }
-  const bool any = open_block(a, b, rest);
-  if (a.unit_mode) b.left = 0;
-  return any;  // (uniform: the range may end before the unit's first tile)
+  return open_block(a, b, rest);  // (uniform: the range may end before the unit's first tile)
 }
 
 // 32 of the D / 2 columns of O that each of a row's two threads has.
@@ -1275,11 +1288,16 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             mx[3] = fmax3_nan(mx[3], sv[c + 6], sv[c + 7]);
           }
         } else {
+          // seen columns as bits: below last + 1, and not below low or below sink
           const int col0 = kv0 + 64 * hc;
-          const int last = my_last - col0, low = my_first - col0, sink = a.sinks - col0;
+          uint32_t seen[2];
+#pragma unroll
+          for (int w = 0; w < 2; ++w)
+            seen[w] = bits_below(my_last + 1 - col0 - 32 * w) &
+                      (~bits_below(my_first - col0 - 32 * w) | bits_below(a.sinks - col0 - 32 * w));
 #pragma unroll
           for (int c = 0; c < 64; ++c) {
-            sv[c] = c <= last && (c >= low || c < sink) ? sv[c] : -INFINITY;
+            sv[c] = seen[c >> 5] & (1u << (c & 31)) ? sv[c] : -INFINITY;
             mx[c & 3] = fmaxf(mx[c & 3], sv[c]);
           }
         }
@@ -1326,7 +1344,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       uint16_t* dst = a.out + static_cast<int64_t>(sg->q0 + sg->tok0 + tok) * a.o_st +
                       static_cast<int64_t>(sg->h * a.G + r % a.G) * a.o_sh + kHalfO * hc;
       const int64_t at = static_cast<int64_t>(2 * blockIdx.x + (sg->begins ? 1 : 0)) * kTileRows + g * kTileM + r;
-#pragma unroll
+#pragma unroll 1  // (code that a CTA runs a few times: fetching it is what it costs)
       for (int c = 0; c < D / 64; ++c) {
         uint32_t o[32];
         if (work > 0) {
@@ -1532,7 +1550,8 @@ static PagedPlan paged_plan(const qik_paged_attn_args& A) {
     const int64_t block = 2 * (kTileM / G), by_rows = A.T / block + A.B, by_seq = A.B * ((A.max_new + block - 1) / block);
     units = (by_rows < by_seq ? by_rows : by_seq) * A.HK;
     work = units * (tiles + kUnitCost);
-    p.unit_mode = tiles <= 8 && units <= 2 * sms;
+    p.unit_mode = tiles <= 8 && units <= 2 * sms && by_seq * A.HK <= 16 * sms;
+    if (p.unit_mode) units = by_seq * A.HK;  // (counted without a look at the lengths)
     p.ctas = sms;
     p.min_share = kUnitCost + 2;
     p.slot_rows = kTileRows;
