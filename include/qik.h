@@ -487,7 +487,7 @@ int qik_add_rms_norm(const void* x, int64_t ldx, const void* residual, int64_t l
                      void* stream);
 
 /*
- * The same with y quantized: scale = max(max|y| * fl32(1/448), 1e-12) over each row
+ * The same with y quantized: scale = max(max|y| / 448, 1e-12) over each row
  * (row_scales != 0: scale [M]) or over the whole tensor (scale [1], the dynamic scale
  * that qik_fp8_gemm takes), q [M, N] = e4m3 (nearest even) of y / scale.  y is not
  * rounded to 16 bits in between; NaN in a row reaches its scale.
