@@ -11,7 +11,9 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <stdarg.h>
@@ -98,6 +100,8 @@ int* status_of(int device) {
   static int* words[64];
   if (device < 0 || device >= 64) refuse(PyExc_ValueError, "qik: device %d is out of range", device);
   if (!words[device]) {
+    // (a first call may come while a graph is captured; status_ptr then keeps clear of it)
+    c10::cuda::CUDAStreamCaptureModeGuard relaxed(cudaStreamCaptureModeRelaxed);
     PyObject* m = PyImport_ImportModule("qik._lib");
     PyObject* p = m ? PyObject_CallMethod(m, "status_ptr", "i", device) : nullptr;
     Py_XDECREF(m);
@@ -347,6 +351,13 @@ PyObject* rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
 }
 
 // ---------------------------------------------------------------- attention
+// (Strided views that interleave in one allocation share no element: torch cannot tell, and they pass.)
+bool overlap(const at::Tensor& a, const at::Tensor& b) {
+  const at::MemOverlapStatus s = at::get_overlap_status(a, b);
+  return s == at::MemOverlapStatus::Full || s == at::MemOverlapStatus::Partial ||
+         (s == at::MemOverlapStatus::TooHard && a.data_ptr() == b.data_ptr());
+}
+
 // paged_attention(q, k_pages, v_pages, page_table, seq_lens, query_starts, max_new, max_kv, sm_scale,
 // causal, window, sinks, out)
 PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
@@ -399,6 +410,9 @@ PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
         refuse(PyExc_ValueError, "qik: out is %s: expected %s", said(o).c_str(), said(q).c_str());
       if (o.stride(2) != 1 || ((o.stride(0) | o.stride(1)) & 7) || !aligned(o))
         refuse(PyExc_ValueError, "qik: out needs a unit column stride, strides of 16 bytes and 16-byte alignment");
+      // a row's place is written while other CTAs still read rows
+      if (at::has_internal_overlap(o) == at::MemOverlap::Yes || overlap(o, q0) || overlap(o, kp) || overlap(o, vp))
+        refuse(PyExc_ValueError, "qik: out overlaps itself, q or the pages");
     }
     const at::Tensor table = table0.stride(1) == 1 || r.W <= 1 ? table0 : table0.contiguous();
     const at::Tensor lens = lens0.contiguous(), starts = starts0.contiguous();

@@ -1532,9 +1532,10 @@ static PagedPlan paged_plan(const qik_paged_attn_args& A) {
   const int sms = sm_count();
   p.split = max_rows <= kSplitRows;
   // the keys that a row can see bound the tiles of a unit
-  const int64_t seen = A.window > 0 && A.window + A.max_new < A.max_kv ? A.window + A.max_new : A.max_kv;
+  const int64_t max_kv = A.max_kv < A.W * A.page ? A.max_kv : A.W * A.page;
+  const int64_t seen = A.window > 0 && A.window + A.max_new < max_kv ? A.window + A.max_new : max_kv;
   const int64_t sinks = A.window > 0 ? A.sinks : 0, size = p.split ? kSplitTile : kTileN;
-  const int64_t tiles = (seen + size - 1) / size + (seen < A.max_kv ? 1 + (sinks + size - 1) / size : 0);
+  const int64_t tiles = (seen + size - 1) / size + (seen < max_kv ? 1 + (sinks + size - 1) / size : 0);
   int64_t units, work, rows = 0;
   if (p.split) {
     p.mt = max_rows <= 16 ? 1 : max_rows <= 32 ? 2 : 4;
@@ -1585,7 +1586,7 @@ static int check_paged(const qik_paged_attn_args& A) {
   QIK_REQUIRE(A.page >= 16 && A.page <= 4096 && (A.page & (A.page - 1)) == 0 && A.pages > 0 && A.pages <= 0x7FFFFFFFll,
               "qik_paged_attention: page of %lld tokens (a power of two, 16 to 4096), %lld pages", (long long)A.page,
               (long long)A.pages);
-  QIK_REQUIRE(A.W >= 0 && A.W * A.page <= (1ll << 30), "qik_paged_attention: page table of %lld columns", (long long)A.W);
+  QIK_REQUIRE(A.W >= 0 && A.W <= (1ll << 30) && A.W * A.page <= (1ll << 30), "qik_paged_attention: page table of %lld columns", (long long)A.W);
   // key tiles of all units are counted in 32 bits
   QIK_REQUIRE(A.HQ / A.HK <= 64, "qik_paged_attention: %lld query heads of one key head (64)", (long long)(A.HQ / A.HK));
   const int64_t blocks = A.T / (kTileM / (A.HQ / A.HK)) + A.B, keys = A.W * A.page;

@@ -187,7 +187,7 @@ using namespace qik;
 extern "C" int qik_rotary(const qik_rotary_args* args, int* status, void* stream) {
   QIK_REQUIRE(args != nullptr, "qik_rotary: args is NULL");
   const qik_rotary_args& A = *args;
-  QIK_REQUIRE(A.T >= 0 && A.HQ >= 0 && A.HK >= 0 && A.HQ + A.HK > 0 && A.HQ <= 4096 && A.HK <= 4096,
+  QIK_REQUIRE(A.T >= 0 && A.T <= 0x7FFFFFFFll && A.HQ >= 0 && A.HK >= 0 && A.HQ + A.HK > 0 && A.HQ <= 4096 && A.HK <= 4096,
               "qik_rotary: bad sizes (T=%lld, %lld + %lld heads)", (long long)A.T, (long long)A.HQ, (long long)A.HK);
   QIK_REQUIRE(A.D == 64 || A.D == 128 || A.D == 256, "qik_rotary: head_dim %lld unsupported (64, 128 or 256)",
               (long long)A.D);
@@ -206,7 +206,7 @@ extern "C" int qik_rotary(const qik_rotary_args* args, int* status, void* stream
               "qik_rotary: strides must be multiples of 8 elements");
   int page_log2 = 0;
   if (paged) {
-    QIK_REQUIRE(A.page > 0 && A.page <= 4096 && (A.page & (A.page - 1)) == 0 && A.pages > 0,
+    QIK_REQUIRE(A.page > 0 && A.page <= 4096 && (A.page & (A.page - 1)) == 0 && A.pages > 0 && A.pages <= 0x7FFFFFFFll,
                 "qik_rotary: page of %lld tokens (a power of two), %lld pages", (long long)A.page, (long long)A.pages);
     QIK_REQUIRE((A.kp_s0 | A.kp_sh | A.kp_ss | A.vp_s0 | A.vp_sh | A.vp_ss) % 8 == 0,
                 "qik_rotary: page strides must be multiples of 8 elements");

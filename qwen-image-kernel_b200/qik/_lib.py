@@ -169,6 +169,12 @@ def status_word(device: torch.device) -> torch.Tensor:
 
 def status_ptr(idx: int) -> int:
     """Address of device ``idx``'s status word (for qik._calls, which keeps it)."""
+    if idx not in _status and torch.cuda.is_current_stream_capturing():
+        # made on the stream that is captured, it would be zeroed at each replay and not before
+        side = torch.cuda.Stream(idx)
+        with torch.cuda.stream(side):
+            status_word(torch.device("cuda", idx))
+        side.synchronize()
     return status_word(torch.device("cuda", idx)).data_ptr()
 
 

@@ -89,6 +89,6 @@ def rotary_store(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: t
     """``apply_rotary`` whose k goes, with v [T, HK, D], into one layer's pages [pages, HK,
     page, D] (page a power of two from 16 to 4096): token t at page slots[t] // page, place
     slots[t] % page.  slots [T] int32 or int64, distinct; a negative slot stores nothing
-    (padding), one behind the last page stores nothing and sets ``STATUS_BAD_INDEX``.  Returns
-    the turned q."""
+    (padding), one behind the last page stores nothing and sets ``STATUS_BAD_INDEX``, and so does
+    a token whose position is outside the table.  Returns the turned q."""
     return _calls.rotary(q, k, v, positions, *table, slots, k_pages, v_pages, interleaved)
