@@ -74,7 +74,7 @@ __device__ __forceinline__ void load_weight8(const void* w, int vec, float (&f)[
 // A code takes the wrong side of a border when the quotient's error is larger than its distance
 // from it, so max|y| / 448 and y / s are products with a rounded reciprocal that one step
 // corrects to half a unit.  (Without it three times as many codes were off by a step; with f32x2
-// arithmetic it costs nothing: 8192 x 3584 took 75.1 us before and 74.0 after.)
+// arithmetic it costs nothing: 8192 x 5120 took 75.1 us before and 74.0 after.)
 __device__ __forceinline__ float norm_scale(uint32_t amax_bits) {
   const float a = __uint_as_float(amax_bits), q = a * (1.0f / 448.0f), r = fmaf(-q, 448.0f, a);
   const float s = r == r ? fmaf(r, 1.0f / 448.0f, q) : q;  // infinity stays
