@@ -1532,7 +1532,7 @@ static PagedPlan paged_plan(const qik_paged_attn_args& A) {
   const int sms = sm_count();
   p.split = max_rows <= kSplitRows;
   // the keys that a row can see bound the tiles of a unit
-  const int64_t max_kv = A.max_kv < A.W * A.page ? A.max_kv : A.W * A.page;
+  const int64_t max_kv = A.max_kv < (1ll << 30) ? A.max_kv : 1ll << 30;  // (no page table holds more)
   const int64_t seen = A.window > 0 && A.window + A.max_new < max_kv ? A.window + A.max_new : max_kv;
   const int64_t sinks = A.window > 0 ? A.sinks : 0, size = p.split ? kSplitTile : kTileN;
   const int64_t tiles = (seen + size - 1) / size + (seen < max_kv ? 1 + (sinks + size - 1) / size : 0);
