@@ -706,6 +706,13 @@ __device__ __forceinline__ float fmax3_nan(float a, float b, float c) {  // NaN 
   return d;
 }
 
+// One lane of the (whole) warp, the same at every call.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
+}
+
 template <int D>
 struct TileShape {
   static constexpr int kHalves = D / 64;
@@ -980,7 +987,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   int* slot = reinterpret_cast<int*>(tmem_slot + 2);  // open_range: 4 + 20 words
   volatile Segment* ring = reinterpret_cast<volatile Segment*>(smem + Sh::kSeg);
 
-  const int warp = threadIdx.x >> 5;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
   const int lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
@@ -1091,81 +1098,102 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     if (n_k > 0 && ok) load_v(n_k - 1);
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer
-    if (lane == 0) {
-      constexpr uint32_t fmt = F16 ? 0 : 1;
-      constexpr uint32_t idesc_s = idesc_f32acc(fmt, fmt, 0, 0, kTileM, kTileN);
-      constexpr uint32_t idesc_o = idesc_f32acc(fmt, fmt, 0, 1, kTileM, D);
-      const uint64_t q_desc = sdesc_sw128(smem_u32(sQ), 16, 1024);
-      const uint64_t k_desc = sdesc_sw128(smem_u32(k_ptr(0)), 16, 1024);
-      const uint64_t v_desc = sdesc_sw128(smem_u32(v_ptr(0)), Sh::kHalfBytes, 1024);
-      constexpr uint64_t kOp16 = Sh::kOperand >> 4;
-      uint32_t base = 0, q_n = 0, p_n[2] = {0u, 0u}, o_n[2] = {0u, 0u};  // tiles, q loads, P and O so far
-      bool ok = true;
-      auto wait = [&](uint64_t* bar, uint32_t parity) { ok = ok && mbar_wait(bar, parity & 1u, abort_flag, a.status); };
-      auto issue_s = [&](int g, uint32_t k) {  // k: the CTA's tile
-        const uint64_t qd = q_desc + g * kOp16, kd = k_desc + static_cast<uint64_t>(k & 1) * kOp16;
+    // The whole warp takes every step and one elected lane issues, from descriptors that are constants of
+    // a stage: so they are warp-uniform values.  (One lane's branch around the loop, with descriptors
+    // computed from the tile's number, was slower to issue than the tensor core to run them: the prompt of 8001
+    // tokens took 460 us, 437 so.)
+    constexpr uint32_t fmt = F16 ? 0 : 1;
+    constexpr uint32_t idesc_s = idesc_f32acc(fmt, fmt, 0, 0, kTileM, kTileN);
+    constexpr uint32_t idesc_o = idesc_f32acc(fmt, fmt, 0, 1, kTileM, D);
+    const uint64_t q_desc = sdesc_sw128(smem_u32(sQ), 16, 1024);
+    const uint64_t k_desc = sdesc_sw128(smem_u32(k_ptr(0)), 16, 1024);
+    const uint64_t v_desc = sdesc_sw128(smem_u32(v_ptr(0)), Sh::kHalfBytes, 1024);
+    constexpr uint64_t kOp16 = Sh::kOperand >> 4;
+    uint32_t base = 0, q_n = 0, p_n[2] = {0u, 0u}, o_n[2] = {0u, 0u};  // tiles, q loads, P and O so far
+    bool ok = true;
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+      ok = ok && __all_sync(0xffffffffu, mbar_wait(bar, parity & 1u, abort_flag, a.status));
+    };
+    auto commit = [&](uint64_t* bar) {
+      if (elect_one()) umma_commit(bar);
+      __syncwarp();
+    };
+    auto s_of = [&](int g, int st) {
+      if (elect_one()) {
 #pragma unroll
         for (int i = 0; i < D / 16; ++i) {
           const uint32_t off16 = ((i >> 2) * Sh::kHalfBytes + (i & 3) * 32) >> 4;
-          umma_f16_ss(tmem + 128u * g, qd + off16, kd + off16, idesc_s, i > 0 ? 1u : 0u);
+          umma_f16_ss(tmem + 128u * g, q_desc + g * kOp16 + off16, k_desc + st * kOp16 + off16, idesc_s, i > 0 ? 1u : 0u);
         }
         umma_commit(&s_full[g]);
-      };
-      auto issue_pv = [&](int g, uint32_t k, bool first) {
-        const uint64_t vd = v_desc + static_cast<uint64_t>(k & 1) * kOp16;
+      }
+      __syncwarp();
+    };
+    auto pv_of = [&](int g, int st, bool first) {
+      if (elect_one()) {
 #pragma unroll
         for (int i = 0; i < kTileN / 16; ++i) {
           const uint32_t p_col = 128u * g + i * 8 + (i >= kTileN / 32 ? 32u : 0u);
-          umma_f16_ts(tmem + 256u + 128u * g, tmem + p_col, vd + i * 128u, idesc_o, !first || i > 0 ? 1u : 0u);
+          umma_f16_ts(tmem + 256u + 128u * g, tmem + p_col, v_desc + st * kOp16 + i * 128u, idesc_o, !first || i > 0 ? 1u : 0u);
         }
-      };
-      for (uint32_t seg = 0; ok && seg_wait(seg); ++seg) {
-        volatile Segment* sg = ring + (seg & (kSegRing - 1));
-        const int n = sg->n, n0 = sg->n0, n1 = sg->n1, most = max(n0, n1);
-        mbar_arrive(&seg_empty[seg & (kSegRing - 1)]);
-        if (n == 0) continue;
-        wait(q_full, q_n++);
-        wait(&k_full[base & 1], base >> 1);
-        tc_fence_after();
-        if (ok) {
-          if (n0 > 0) issue_s(0, base);
-          if (n1 > 0) issue_s(1, base);
-          umma_commit(&k_empty[base & 1]);
-          if (most <= 1) umma_commit(q_empty);
-        }
-        for (int t = 0; t < n && ok; ++t) {
-          const uint32_t k = base + t;
+      }
+      __syncwarp();
+    };
+    auto issue_s = [&](int g, uint32_t k) {  // k: the CTA's tile
+      if (k & 1) s_of(g, 1);
+      else s_of(g, 0);
+    };
+    auto issue_pv = [&](int g, uint32_t k, bool first) {
+      if (k & 1) pv_of(g, 1, first);
+      else pv_of(g, 0, first);
+    };
+    for (uint32_t seg = 0; ok && __all_sync(0xffffffffu, seg_wait(seg)); ++seg) {
+      volatile Segment* sg = ring + (seg & (kSegRing - 1));
+      const int n = sg->n, n0 = sg->n0, n1 = sg->n1, most = max(n0, n1);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&seg_empty[seg & (kSegRing - 1)]);
+      if (n == 0) continue;
+      wait(q_full, q_n++);
+      wait(&k_full[base & 1], base >> 1);
+      tc_fence_after();
+      if (ok) {
+        if (n0 > 0) issue_s(0, base);
+        if (n1 > 0) issue_s(1, base);
+        commit(&k_empty[base & 1]);
+        if (most <= 1) commit(q_empty);
+      }
+      for (int t = 0; t < n && ok; ++t) {
+        const uint32_t k = base + t;
 #pragma unroll
-          for (int g = 0; g < 2; ++g) {  // (unrolled: p_n and o_n stay in registers)
-            const int mine = g == 0 ? n0 : n1;
-            if (ok && t < mine) {
-              wait(&p_full[g], p_n[g]++);
-              if (g == 0 || n0 <= t) wait(&v_full[k & 1], k >> 1);
-              if (t == 0 && o_n[g] > 0) wait(&o_empty[g], o_n[g] - 1);
-              if (ok) {
-                tc_fence_after();
-                issue_pv(g, k, t == 0);
-                if (t == mine - 1) {
-                  umma_commit(&o_full[g]);
-                  ++o_n[g];
-                }
+        for (int g = 0; g < 2; ++g) {  // (unrolled: p_n and o_n stay in registers)
+          const int mine = g == 0 ? n0 : n1;
+          if (ok && t < mine) {
+            wait(&p_full[g], p_n[g]++);
+            if (g == 0 || n0 <= t) wait(&v_full[k & 1], k >> 1);
+            if (t == 0 && o_n[g] > 0) wait(&o_empty[g], o_n[g] - 1);
+            if (ok) {
+              tc_fence_after();
+              issue_pv(g, k, t == 0);
+              if (t == mine - 1) {
+                commit(&o_full[g]);
+                ++o_n[g];
               }
-            }
-            if (g == 1 && ok) umma_commit(&v_empty[k & 1]);
-            if (ok && t + 1 < mine) {
-              if (g == 0 || n0 <= t + 1) {
-                wait(&k_full[(k + 1) & 1], (k + 1) >> 1);
-                tc_fence_after();
-              }
-              if (ok) issue_s(g, k + 1);
             }
           }
-          if (!ok) break;
-          if (t + 1 < n) umma_commit(&k_empty[(k + 1) & 1]);
-          if (most > 1 && t + 2 == most) umma_commit(q_empty);
+          if (g == 1 && ok) commit(&v_empty[k & 1]);
+          if (ok && t + 1 < mine) {
+            if (g == 0 || n0 <= t + 1) {
+              wait(&k_full[(k + 1) & 1], (k + 1) >> 1);
+              tc_fence_after();
+            }
+            if (ok) issue_s(g, k + 1);
+          }
         }
-        base += n;
+        if (!ok) break;
+        if (t + 1 < n) commit(&k_empty[(k + 1) & 1]);
+        if (most > 1 && t + 2 == most) commit(q_empty);
       }
+      base += n;
     }
   } else if (warp == 2) {
     // ------------------------------------------------------------ V rows nobody sees
