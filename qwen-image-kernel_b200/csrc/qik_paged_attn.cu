@@ -695,7 +695,8 @@ constexpr int kTileRows = 2 * kTileM;          // rows of a CTA
 constexpr int kTileSoftmaxWarps = 8;           // per query tile: two threads a row
 constexpr int kTileThreads = 128 + 64 * kTileSoftmaxWarps;
 constexpr float kTileRescale = 8.0f;           // O is rescaled when a maximum grows by > 2^8
-constexpr int kTilePolyFrom = 23;              // pairs of a half row from here on take 2^x on the FMA pipe
+constexpr int kTilePolyFrom0 = 12;             // pairs of a part from here on take 2^x on the FMA pipe
+constexpr int kTilePolyFrom1 = 11;
 
 __device__ __forceinline__ uint32_t bits_below(int n) {  // the lowest n bits, n clamped to [0, 32]
   return n >= 32 ? 0xFFFFFFFFu : n <= 0 ? 0u : (1u << n) - 1u;
@@ -909,18 +910,17 @@ __device__ __forceinline__ void tmem_st_cols(uint32_t addr, const uint32_t (&r)[
   else tmem_st_2x32_at32(addr, r);
 }
 
-// P half row: the thread's 64 scores, p = 2^(s * scale - m) in pairs, packed over its own
-// S columns (as qik_attn.cu's softmax_half_row); returns the half row's fp32 sum.
-template <bool kPoly, bool F16>
-__device__ __forceinline__ float tile_softmax(const float (&sv)[64], float scale, float neg_m, uint32_t tP) {
+// Part H of a P half row: 32 of the thread's 64 scores, p = 2^(s * scale - m) in pairs, packed over
+// its own S columns (as qik_attn.cu's softmax_half_row); their fp32 sums are added to acc.
+template <bool kPoly, bool F16, int H>
+__device__ __forceinline__ void tile_softmax(const float (&sv)[64], float scale, float neg_m, uint32_t tP, uint64_t (&acc)[2]) {
   const uint64_t sc2 = f2_pack(scale, scale), nm2 = f2_pack(neg_m, neg_m);
-  uint64_t acc[2] = {0ull, 0ull};
-  uint32_t pk[32];
+  uint32_t pk[16];
 #pragma unroll
-  for (int j = 0; j < 32; ++j) {
-    const uint64_t x2 = ffma2(f2_pack(sv[2 * j], sv[2 * j + 1]), sc2, nm2);
+  for (int j = 0; j < 16; ++j) {
+    const uint64_t x2 = ffma2(f2_pack(sv[32 * H + 2 * j], sv[32 * H + 2 * j + 1]), sc2, nm2);
     uint64_t p2;
-    if (kPoly && j >= kTilePolyFrom) {
+    if (kPoly && j >= (H ? kTilePolyFrom1 : kTilePolyFrom0)) {
       p2 = exp2_poly2(x2);
     } else {
       float x0, x1;
@@ -933,8 +933,7 @@ __device__ __forceinline__ float tile_softmax(const float (&sv)[64], float scale
     pk[j] = pack16<F16>(p0, p1);
   }
   __syncwarp();
-  tmem_st_2x32(tP, pk);
-  return f2_sum(acc[0]) + f2_sum(acc[1]);
+  tmem_st_2x16(tP + 16 * H, pk);
 }
 
 // What the warps know of a segment, in a ring in shared memory: kept there so that the softmax
@@ -982,7 +981,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   uint64_t* o_empty = bars + 18;  // [tile] O has been read
   uint64_t* seg_full = bars + 20;   // [kSegRing]
   uint64_t* seg_empty = bars + 24;  // [kSegRing]
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 28);
+  uint64_t* h_full = bars + 28;   // [tile] the first 32 keys of each half of P
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 30);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int* slot = reinterpret_cast<int*>(tmem_slot + 2);  // open_range: 4 + 20 words
   volatile Segment* ring = reinterpret_cast<volatile Segment*>(smem + Sh::kSeg);
@@ -999,6 +999,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       mbar_init(&v_raw[s], 1);
       mbar_init(&v_empty[s], 1);
       mbar_init(&s_full[s], 1);
+      mbar_init(&h_full[s], kTileSoftmaxWarps);
       mbar_init(&p_full[s], kTileSoftmaxWarps);
       mbar_init(&o_full[s], 1);
       mbar_init(&o_empty[s], kTileSoftmaxWarps);
@@ -1129,12 +1130,13 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       }
       __syncwarp();
     };
-    auto pv_of = [&](int g, int st, bool first) {
+    auto pv_of = [&](int g, int st, int part, bool first) {  // 32 keys of each half of P
       if (elect_one()) {
 #pragma unroll
-        for (int i = 0; i < kTileN / 16; ++i) {
+        for (int j = 0; j < kTileN / 32; ++j) {
+          const int i = 2 * part + (j & 1) + (j >> 1) * (kTileN / 32);
           const uint32_t p_col = 128u * g + i * 8 + (i >= kTileN / 32 ? 32u : 0u);
-          umma_f16_ts(tmem + 256u + 128u * g, tmem + p_col, v_desc + st * kOp16 + i * 128u, idesc_o, !first || i > 0 ? 1u : 0u);
+          umma_f16_ts(tmem + 256u + 128u * g, tmem + p_col, v_desc + st * kOp16 + i * 128u, idesc_o, !first || j > 0 ? 1u : 0u);
         }
       }
       __syncwarp();
@@ -1143,9 +1145,9 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       if (k & 1) s_of(g, 1);
       else s_of(g, 0);
     };
-    auto issue_pv = [&](int g, uint32_t k, bool first) {
-      if (k & 1) pv_of(g, 1, first);
-      else pv_of(g, 0, first);
+    auto issue_pv = [&](int g, uint32_t k, int part, bool first) {
+      if (k & 1) pv_of(g, 1, part, first);
+      else pv_of(g, 0, part, first);
     };
     for (uint32_t seg = 0; ok && __all_sync(0xffffffffu, seg_wait(seg)); ++seg) {
       volatile Segment* sg = ring + (seg & (kSegRing - 1));
@@ -1168,12 +1170,17 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         for (int g = 0; g < 2; ++g) {  // (unrolled: p_n and o_n stay in registers)
           const int mine = g == 0 ? n0 : n1;
           if (ok && t < mine) {
-            wait(&p_full[g], p_n[g]++);
+            wait(&h_full[g], p_n[g]);
             if (g == 0 || n0 <= t) wait(&v_full[k & 1], k >> 1);
             if (t == 0 && o_n[g] > 0) wait(&o_empty[g], o_n[g] - 1);
             if (ok) {
               tc_fence_after();
-              issue_pv(g, k, t == 0);
+              issue_pv(g, k, 0, t == 0);
+              wait(&p_full[g], p_n[g]++);
+            }
+            if (ok) {
+              tc_fence_after();
+              issue_pv(g, k, 1, false);
               if (t == mine - 1) {
                 commit(&o_full[g]);
                 ++o_n[g];
@@ -1341,9 +1348,11 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           m_run = tmax;
         }
         const float neg_m = m_run == -INFINITY ? 0.0f : -m_run;
-        const float psum = whole ? tile_softmax<true, F16>(sv, a.scale_log2, neg_m, tS)
-                                 : tile_softmax<false, F16>(sv, a.scale_log2, neg_m, tS);
-        l_run = l_run * alpha + (raw_max == raw_max ? psum : raw_max);
+        uint64_t acc[2] = {0ull, 0ull};
+        if (whole)
+          tile_softmax<true, F16, 0>(sv, a.scale_log2, neg_m, tS, acc);
+        else
+          tile_softmax<false, F16, 0>(sv, a.scale_log2, neg_m, tS, acc);
         if (t >= 1 && __any_sync(0xffffffffu, rescale)) {
           const float f = rescale ? alpha : 1.0f;
 #pragma unroll
@@ -1355,6 +1364,15 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             tmem_st_cols<D>(tO + c * 32, rr);
           }
         }
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&h_full[g]);
+        if (whole)
+          tile_softmax<true, F16, 1>(sv, a.scale_log2, neg_m, tS, acc);
+        else
+          tile_softmax<false, F16, 1>(sv, a.scale_log2, neg_m, tS, acc);
+        l_run = l_run * alpha + (raw_max == raw_max ? f2_sum(acc[0]) + f2_sum(acc[1]) : raw_max);
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
