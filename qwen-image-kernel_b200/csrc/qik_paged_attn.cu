@@ -695,16 +695,10 @@ constexpr int kTileRows = 2 * kTileM;          // rows of a CTA
 constexpr int kTileSoftmaxWarps = 8;           // per query tile: two threads a row
 constexpr int kTileThreads = 128 + 64 * kTileSoftmaxWarps;
 constexpr float kTileRescale = 8.0f;           // O is rescaled when a maximum grows by > 2^8
-constexpr int kTilePolyFrom0 = 12;             // pairs of a part from here on take 2^x on the FMA pipe
-constexpr int kTilePolyFrom1 = 11;
+constexpr int kTileSplitP = 2;                 // steps of 16 keys of each half of P handed over first (1, 3: 427 us)
 
 __device__ __forceinline__ uint32_t bits_below(int n) {  // the lowest n bits, n clamped to [0, 32]
   return n >= 32 ? 0xFFFFFFFFu : n <= 0 ? 0u : (1u << n) - 1u;
-}
-__device__ __forceinline__ float fmax3_nan(float a, float b, float c) {  // NaN if any is
-  float d;
-  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-  return d;
 }
 
 // One lane of the (whole) warp, the same at every call.
@@ -910,30 +904,27 @@ __device__ __forceinline__ void tmem_st_cols(uint32_t addr, const uint32_t (&r)[
   else tmem_st_2x32_at32(addr, r);
 }
 
-// Part H of a P half row: 32 of the thread's 64 scores, p = 2^(s * scale - m) in pairs, packed over
-// its own S columns (as qik_attn.cu's softmax_half_row); their fp32 sums are added to acc.
-template <bool kPoly, bool F16, int H>
+// Steps [FROM, TO) of 16 keys of a P half row: p = 2^(s * scale - m) of the thread's scores in pairs,
+// packed over its own S columns; their fp32 sums are added to acc.  (2^x of some pairs on the
+// FMA pipe, as qik_attn.cu does it, did not pay: the prompt of 8001 tokens took 417 us without, 421 with
+// 9 of 32 pairs there, 428 with 13.)
+template <bool F16, int FROM, int TO>
 __device__ __forceinline__ void tile_softmax(const float (&sv)[64], float scale, float neg_m, uint32_t tP, uint64_t (&acc)[2]) {
   const uint64_t sc2 = f2_pack(scale, scale), nm2 = f2_pack(neg_m, neg_m);
-  uint32_t pk[16];
 #pragma unroll
-  for (int j = 0; j < 16; ++j) {
-    const uint64_t x2 = ffma2(f2_pack(sv[32 * H + 2 * j], sv[32 * H + 2 * j + 1]), sc2, nm2);
-    uint64_t p2;
-    if (kPoly && j >= (H ? kTilePolyFrom1 : kTilePolyFrom0)) {
-      p2 = exp2_poly2(x2);
-    } else {
+  for (int i = FROM; i < TO; ++i) {
+    uint32_t pk[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
       float x0, x1;
-      f2_unpack(x2, x0, x1);
-      p2 = f2_pack(ex2(x0), ex2(x1));
+      f2_unpack(ffma2(f2_pack(sv[16 * i + 2 * j], sv[16 * i + 2 * j + 1]), sc2, nm2), x0, x1);
+      const float p0 = ex2(x0), p1 = ex2(x1);
+      acc[j & 1] = fadd2(acc[j & 1], f2_pack(p0, p1));
+      pk[j] = pack16<F16>(p0, p1);
     }
-    acc[j & 1] = fadd2(acc[j & 1], p2);
-    float p0, p1;
-    f2_unpack(p2, p0, p1);
-    pk[j] = pack16<F16>(p0, p1);
+    if (i == 0) __syncwarp();
+    tmem_st_2x8(tP + 8 * i, pk);
   }
-  __syncwarp();
-  tmem_st_2x16(tP + 16 * H, pk);
 }
 
 // What the warps know of a segment, in a ring in shared memory: kept there so that the softmax
@@ -1130,13 +1121,14 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       }
       __syncwarp();
     };
-    auto pv_of = [&](int g, int st, int part, bool first) {  // 32 keys of each half of P
+    auto pv_of = [&](int g, int st, int part, bool first) {  // the steps of a part, of each half of P
       if (elect_one()) {
 #pragma unroll
-        for (int j = 0; j < kTileN / 32; ++j) {
-          const int i = 2 * part + (j & 1) + (j >> 1) * (kTileN / 32);
-          const uint32_t p_col = 128u * g + i * 8 + (i >= kTileN / 32 ? 32u : 0u);
-          umma_f16_ts(tmem + 256u + 128u * g, tmem + p_col, v_desc + st * kOp16 + i * 128u, idesc_o, !first || j > 0 ? 1u : 0u);
+        for (int j = 0; j < kTileN / 16; ++j) {
+          const int half = j / 4, i = j % 4;
+          if ((i < kTileSplitP) != (part == 0)) continue;
+          umma_f16_ts(tmem + 256u + 128u * g, tmem + 128u * g + 64u * half + 8u * i, v_desc + st * kOp16 + j * 128u, idesc_o,
+                      !first || j > 0 ? 1u : 0u);
         }
       }
       __syncwarp();
@@ -1317,10 +1309,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         if (whole) {
 #pragma unroll
           for (int c = 0; c < 64; c += 8) {
-            mx[0] = fmax3_nan(mx[0], sv[c], sv[c + 1]);
-            mx[1] = fmax3_nan(mx[1], sv[c + 2], sv[c + 3]);
-            mx[2] = fmax3_nan(mx[2], sv[c + 4], sv[c + 5]);
-            mx[3] = fmax3_nan(mx[3], sv[c + 6], sv[c + 7]);
+            mx[0] = fmaxf(fmaxf(mx[0], sv[c]), sv[c + 1]);
+            mx[1] = fmaxf(fmaxf(mx[1], sv[c + 2]), sv[c + 3]);
+            mx[2] = fmaxf(fmaxf(mx[2], sv[c + 4]), sv[c + 5]);
+            mx[3] = fmaxf(fmaxf(mx[3], sv[c + 6]), sv[c + 7]);
           }
         } else {
           // seen columns as bits: below last + 1, and not below low or below sink
@@ -1336,9 +1328,9 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             mx[c & 3] = fmaxf(mx[c & 3], sv[c]);
           }
         }
-        // a NaN score reaches the row's sum through its maximum: 2^x on the FMA pipe clamps it
-        float raw_max = fmax3_nan(mx[0], mx[1], mx[2]);
-        raw_max = fmax3_nan(raw_max, mx[3], __shfl_xor_sync(0xffffffffu, fmax3_nan(raw_max, mx[3], mx[3]), 16));
+        // (NaN scores do not reach the maximum; they reach P and the sum)
+        float raw_max = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+        raw_max = fmaxf(raw_max, __shfl_xor_sync(0xffffffffu, raw_max, 16));
         const float tmax = raw_max * a.scale_log2;
         float alpha = 1.0f;
         bool rescale = false;
@@ -1349,10 +1341,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         }
         const float neg_m = m_run == -INFINITY ? 0.0f : -m_run;
         uint64_t acc[2] = {0ull, 0ull};
-        if (whole)
-          tile_softmax<true, F16, 0>(sv, a.scale_log2, neg_m, tS, acc);
-        else
-          tile_softmax<false, F16, 0>(sv, a.scale_log2, neg_m, tS, acc);
+        tile_softmax<F16, 0, kTileSplitP>(sv, a.scale_log2, neg_m, tS, acc);
         if (t >= 1 && __any_sync(0xffffffffu, rescale)) {
           const float f = rescale ? alpha : 1.0f;
 #pragma unroll
@@ -1368,11 +1357,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&h_full[g]);
-        if (whole)
-          tile_softmax<true, F16, 1>(sv, a.scale_log2, neg_m, tS, acc);
-        else
-          tile_softmax<false, F16, 1>(sv, a.scale_log2, neg_m, tS, acc);
-        l_run = l_run * alpha + (raw_max == raw_max ? f2_sum(acc[0]) + f2_sum(acc[1]) : raw_max);
+        tile_softmax<F16, kTileSplitP, 4>(sv, a.scale_log2, neg_m, tS, acc);
+        l_run = l_run * alpha + (f2_sum(acc[0]) + f2_sum(acc[1]));
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
