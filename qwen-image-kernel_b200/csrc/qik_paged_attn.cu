@@ -1045,7 +1045,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     uint32_t n_k = 0;  // tiles issued so far
     // the previous tile, whose V is still to be loaded
     int v_id = -1, v_place = 0, v_h = 0;
-    bool v_edge = false, ok = true;
+    bool v_owed = false, v_edge = false, ok = true;
     auto load = [&](const CUtensorMap* tm, uint8_t* dst, int id, int place, int h, uint64_t* bar) {
       if (lane == 0) mbar_arrive_expect_tx(bar, Sh::kOperand);
       __syncwarp();
@@ -1055,10 +1055,12 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           tma_load_5d(dst + hd * Sh::kHalfBytes + lane * box * 128, tm, 0, place, hd, h, id, bar);
       }
     };
-    auto load_v = [&](uint32_t t) {  // V of tile t of the CTA
-      const int st = t & 1;
-      ok = ok && __all_sync(0xffffffffu, mbar_wait(&v_empty[st], ((t >> 1) & 1) ^ 1u, abort_flag, a.status));
+    auto load_v = [&]() {  // V of the last tile issued, where it is still owed
+      if (!v_owed) return;
+      const int st = (n_k - 1) & 1;
+      ok = ok && __all_sync(0xffffffffu, mbar_wait(&v_empty[st], (((n_k - 1) >> 1) & 1) ^ 1u, abort_flag, a.status));
       if (ok) load(&tm_v, v_ptr(st), v_id, v_place, v_h, v_edge ? &v_raw[st] : &v_full[st]);
+      v_owed = false;
     };
     for (uint32_t seg = 0; ok && __all_sync(0xffffffffu, seg_wait(seg)); ++seg) {
       volatile Segment* sg = ring + (seg & (kSegRing - 1));
@@ -1067,6 +1069,9 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       const int32_t* row = a.table + static_cast<int64_t>(sg->i) * a.table_st;
       __syncwarp();
       if (lane == 0) mbar_arrive(&seg_empty[seg & (kSegRing - 1)]);
+      // A segment without keys issues no K that V could follow, and with kSegRing - 1 of them in a row
+      // the ring stays full until the softmax of the segment before them has its last V.
+      if (n == 0) load_v();
       auto page_of = [&](int first) {
         if (lane >= pieces) return -1;
         const int key = first + lane * box;
@@ -1084,12 +1089,13 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         ok = __all_sync(0xffffffffu, mbar_wait(&k_empty[st], ((n_k >> 1) & 1) ^ 1u, abort_flag, a.status));
         if (!ok) break;
         load(&tm_k, k_ptr(st), id, place, h, &k_full[st]);
-        if (n_k > 0) load_v(n_k - 1);
+        load_v();
+        v_owed = true;
         v_id = id, v_place = place, v_h = h, v_edge = edge(kv0, lmin, lmax);
         kv0 = kv1;
       }
     }
-    if (n_k > 0 && ok) load_v(n_k - 1);
+    if (ok) load_v();
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer
     // The whole warp takes every step and one elected lane issues, from descriptors that are constants of
