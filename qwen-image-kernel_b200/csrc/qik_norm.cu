@@ -274,6 +274,7 @@ __global__ void __launch_bounds__(1024) __cluster_dims__(kNormCluster, 1, 1) add
   __shared__ uint32_t tops[kNormCluster];  // every CTA's max|y| bits, written by their owners
   const int nv = a.N >> 3;
   const uint32_t rank = cluster_ctarank();
+  cluster_arrive_started();
   pdl_wait();
   float h[kNormClusterRows][VPT][8];
   uint4 xv[kNormClusterRows][VPT], rv[kNormClusterRows][VPT];
@@ -327,6 +328,7 @@ __global__ void __launch_bounds__(1024) __cluster_dims__(kNormCluster, 1, 1) add
     }
   }
   top = block_reduce<true>(top, red[kNormClusterRows]);
+  cluster_wait_started();  // (behind the loads: a CTA without rows gets here at once, ahead of its peers)
   if (threadIdx.x < kNormCluster) st_cluster_u32(mapa_shared(&tops[rank], threadIdx.x), top);
   cluster_sync();
   uint32_t m = 0;
