@@ -34,7 +34,7 @@
 // whatever an unused place of a page holds.  Where a row's result is not finite and a key that
 // it does not see, but other rows of its tile do, has infinities or NaN in V, the row is computed
 // again from the keys that it sees (mend_row, a path that finite values never take): a row's
-// result depends on what it sees alone.
+// result depends on what it sees alone.  The CTA's waits know of it (paged_wait).
 #include <mutex>
 #include <type_traits>
 
@@ -112,72 +112,130 @@ template <bool F16>
 __device__ __forceinline__ float to_float(uint32_t half) {
   return F16 ? __half2float(__ushort_as_half(static_cast<unsigned short>(half))) : __uint_as_float(half << 16);
 }
-// A row whose sums o (NC pairs of columns, the first two at `col`, the next ones `step` columns on,
-// in units of 2^m) are not all finite: if some key of the tiles [u0, u1) that the row does not see
-// and that is not zeroed for all rows has infinities or NaN in V, the sums are formed again, key
-// by key, from those that it sees.  Whatever else makes a sum infinite or NaN stays.
-template <int D, bool F16, int TILE, int NC>
-__device__ __forceinline__ void mend_row(const PagedDev& a, float (&o)[NC][2], int col, int step, const Tiles& t, int u0, int u1,
-                                         int seq, int h, int row, int hq, int last, int first, float m) {
-  bool bad = false;
+// Bounded wait (mbar_wait) whose limit starts again while warps of the CTA form rows again:
+// flags[0] says that a wait gave up, flags[1] how many warps are in mend_row.  That takes as long as a
+// row has keys, with the pipeline's other roles waiting.
+__device__ __forceinline__ bool paged_wait(uint64_t* bar, uint32_t parity, volatile int* flags, int* status) {
+  if (mbar_try_wait(bar, parity)) return true;
+  uint64_t t0 = globaltimer();
+  for (uint32_t it = 1;; ++it) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if ((it & 63u) == 0u) {
+      if (flags[0]) return false;
+      const uint64_t now = globaltimer();
+      if (flags[1] > 0) t0 = now;
+      if (now - t0 > QIK_WAIT_NS) {
+        flags[0] = 1;
+        if (status) atomicExch(status, QIK_DEV_TIMEOUT);
+        return false;
+      }
+    }
+  }
+}
+
+template <bool F16>
+__device__ __forceinline__ float dot8(const uint4& x, const uint4& y, float s) {
+  const uint32_t a[4] = {x.x, x.y, x.z, x.w}, b[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
-  for (int c = 0; c < NC; ++c) bad = bad || !isfinite(o[c][0]) || !isfinite(o[c][1]);
-  if (!bad) return;
+  for (int i = 0; i < 4; ++i) {
+    s = fmaf(to_float<F16>(a[i] & 0xFFFFu), to_float<F16>(b[i] & 0xFFFFu), s);
+    s = fmaf(to_float<F16>(a[i] >> 16), to_float<F16>(b[i] >> 16), s);
+  }
+  return s;
+}
+// Columns of o that are not finite, as bits 2c and 2c + 1 of pair c; `nan_only`: that are NaN.
+template <int NC>
+__device__ __forceinline__ uint32_t odd_columns(const float (&o)[NC][2], bool nan_only) {
+  uint32_t r = 0;
+#pragma unroll
+  for (int c = 0; c < NC; ++c)
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      if (nan_only ? isnan(o[c][i]) : !isfinite(o[c][i])) r |= 1u << (2 * c + i);
+  return r;
+}
+// A row whose sums o (NC pairs of columns, the first two at `col`, the next ones `step` columns on,
+// in units of 2^m) are not all finite: a column in which some key of the tiles [u0, u1) that the
+// row does not see, and that is not zeroed for all rows, has infinities or NaN in V is formed
+// again, key by key, from those that the row sees.  Whatever else makes a sum infinite or NaN stays.
+// The keys are taken from the last one down, until every such column is NaN: where NaN has spread
+// over a sequence, a row sees it at its own place, and this ends after one key.  (A column of
+// infinities goes through all of them.)
+template <int D, bool F16, int TILE, int NC>
+__device__ __noinline__ void mend_row(const PagedDev& a, float (&o)[NC][2], int col, int step, Tiles t, int u0, int u1,
+                                     int seq, int h, int row, int hq, int last, int first, float m) {
+  static_assert(NC <= 16, "columns as bits of a word");
+  const uint32_t odd = odd_columns(o, false);
+  if (!odd) return;
   const int32_t* table = a.table + static_cast<int64_t>(seq) * a.table_st;
   auto page_at = [&](int kv) -> int64_t {
     const int at = kv >> a.page_log2, id = at < a.W ? __ldg(table + at) : -1;
     return id < a.pages ? id : -1;
   };
-  auto value = [&](int64_t page, int kv, int c) {
-    return __ldg(reinterpret_cast<const uint32_t*>(a.v_pages + page * a.vp_s0 + h * a.vp_sh +
-                                                   (kv & ((1 << a.page_log2) - 1)) * a.vp_ss + col + c * step));
+  auto v_at = [&](int64_t page, int kv) {
+    return reinterpret_cast<const uint32_t*>(a.v_pages + page * a.vp_s0 + h * a.vp_sh +
+                                             (kv & ((1 << a.page_log2) - 1)) * a.vp_ss + col);
   };
   auto sees = [&](int kv) { return kv <= last && (kv >= first || kv < a.sinks); };
-  bad = false;
+  uint32_t spoilt = 0;
 #pragma unroll 1
-  for (int u = u0; u < u1 && !bad; ++u) {
+  for (int u = u1 - 1; u >= u0 && spoilt != odd; --u) {
     const int kv0 = tile_at(t, u) * TILE;
     if (kv0 + TILE - 1 <= last && (kv0 >= first || kv0 + TILE - 1 < a.sinks)) continue;
 #pragma unroll 1
-    for (int kv = kv0; kv < kv0 + TILE && !bad; ++kv) {
+    for (int kv = kv0; kv < kv0 + TILE && spoilt != odd; ++kv) {
       if (sees(kv) || kv > t.lmax || (kv < t.lmin && kv >= a.sinks)) continue;
       const int64_t page = page_at(kv);
-#pragma unroll 1
-      for (int c = 0; c < NC && page >= 0; ++c) {
-        const uint32_t w = value(page, kv, c);
-        bad = bad || !isfinite(to_float<F16>(w & 0xFFFFu)) || !isfinite(to_float<F16>(w >> 16));
-      }
-    }
-  }
-  if (!bad) return;
-#pragma unroll
-  for (int c = 0; c < NC; ++c) o[c][0] = o[c][1] = 0.0f;
-  const uint32_t* q = reinterpret_cast<const uint32_t*>(a.q + static_cast<int64_t>(row) * a.q_st + static_cast<int64_t>(hq) * a.q_sh);
-#pragma unroll 1
-  for (int u = u0; u < u1; ++u) {
-    const int kv0 = tile_at(t, u) * TILE;
-#pragma unroll 1
-    for (int kv = kv0; kv < kv0 + TILE; ++kv) {
-      const int64_t page = sees(kv) ? page_at(kv) : -1;
-      if (page < 0) continue;  // (a page outside the pool reads zeros: it adds nothing)
-      const uint32_t* k = reinterpret_cast<const uint32_t*>(a.k_pages + page * a.kp_s0 + h * a.kp_sh +
-                                                            (kv & ((1 << a.page_log2) - 1)) * a.kp_ss);
-      float s = 0.0f;
-#pragma unroll 1
-      for (int d = 0; d < D / 2; ++d) {
-        const uint32_t x = __ldg(q + d), y = __ldg(k + d);
-        s = fmaf(to_float<F16>(x & 0xFFFFu), to_float<F16>(y & 0xFFFFu), s);
-        s = fmaf(to_float<F16>(x >> 16), to_float<F16>(y >> 16), s);
-      }
-      const float p = ex2(fmaf(s, a.scale_log2, -m));
+      if (page < 0) continue;
+      const uint32_t* v = v_at(page, kv);
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
-        const uint32_t w = value(page, kv, c);
-        o[c][0] = fmaf(p, to_float<F16>(w & 0xFFFFu), o[c][0]);
-        o[c][1] = fmaf(p, to_float<F16>(w >> 16), o[c][1]);
+        const uint32_t w = __ldg(v + c * (step / 2));
+        if (!isfinite(to_float<F16>(w & 0xFFFFu))) spoilt |= odd & (1u << (2 * c));
+        if (!isfinite(to_float<F16>(w >> 16))) spoilt |= odd & (2u << (2 * c));
       }
     }
   }
+  if (!spoilt) return;
+#pragma unroll
+  for (int c = 0; c < NC; ++c)
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      if (spoilt & (1u << (2 * c + i))) o[c][i] = 0.0f;
+  const uint4* q = reinterpret_cast<const uint4*>(a.q + static_cast<int64_t>(row) * a.q_st + static_cast<int64_t>(hq) * a.q_sh);
+  bool open = true;
+#pragma unroll 1
+  for (int u = u1 - 1; u >= u0 && open; --u) {
+    const int kv0 = tile_at(t, u) * TILE;
+#pragma unroll 1
+    for (int kv = kv0 + TILE - 1; kv >= kv0 && open; --kv) {
+      const int64_t page = sees(kv) ? page_at(kv) : -1;
+      if (page < 0) continue;  // (a page outside the pool reads zeros: it adds nothing)
+      const uint4* k = reinterpret_cast<const uint4*>(a.k_pages + page * a.kp_s0 + h * a.kp_sh +
+                                                      (kv & ((1 << a.page_log2) - 1)) * a.kp_ss);
+      float s = 0.0f;
+#pragma unroll 1
+      for (int d = 0; d < D / 8; ++d) s = dot8<F16>(__ldg(q + d), __ldg(k + d), s);
+      const float p = ex2(fmaf(s, a.scale_log2, -m));
+      const uint32_t* v = v_at(page, kv);
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        const uint32_t w = __ldg(v + c * (step / 2));
+        if (spoilt & (1u << (2 * c))) o[c][0] = fmaf(p, to_float<F16>(w & 0xFFFFu), o[c][0]);
+        if (spoilt & (2u << (2 * c))) o[c][1] = fmaf(p, to_float<F16>(w >> 16), o[c][1]);
+      }
+      open = (spoilt & ~odd_columns(o, true)) != 0;
+    }
+  }
+}
+// Calls mend() in the lanes of a whole warp whose row is `odd`; the CTA's waits know of it.
+template <typename Mend>
+__device__ __forceinline__ void mend_rows(volatile int* flags, bool odd, Mend mend) {
+  if (!__any_sync(0xffffffffu, odd)) return;
+  if ((threadIdx.x & 31) == 0) atomicAdd(const_cast<int*>(flags + 1), 1);
+  if (odd) mend();
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) atomicSub(const_cast<int*>(flags + 1), 1);
 }
 
 // ============================================================ few rows: split over keys
@@ -291,13 +349,13 @@ __device__ __forceinline__ bool walk_next(const PagedDev& a, Walk& w, int taken)
 template <int D, int MT, int TEAMS, bool F16>
 __global__ void __launch_bounds__(SplitShape<D, MT, TEAMS>::kThreads, SplitShape<D, MT, TEAMS>::kCtasPerSm)
     paged_split_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
-                       const PagedDev a) {
+                       const __grid_constant__ PagedDev a) {
   using Sh = SplitShape<D, MT, TEAMS>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + Sh::kBar);
   uint64_t* empty = full + Sh::kStages;
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(empty + Sh::kStages);
+  volatile int* flags = reinterpret_cast<volatile int*>(empty + Sh::kStages);
   volatile int* scan = reinterpret_cast<volatile int*>(smem + Sh::kMerge);  // before the merge buffer is used
   volatile int* found = reinterpret_cast<volatile int*>(smem + Sh::kMl);
 
@@ -307,7 +365,7 @@ __global__ void __launch_bounds__(SplitShape<D, MT, TEAMS>::kThreads, SplitShape
       mbar_init(&full[s], 2);  // the K and the V producer
       mbar_init(&empty[s], Sh::kWarps / Sh::kTeams);
     }
-    *abort_flag = 0;
+    flags[0] = flags[1] = 0;
     found[0] = a.B;
     fence_mbar_init();
   }
@@ -428,7 +486,7 @@ __global__ void __launch_bounds__(SplitShape<D, MT, TEAMS>::kThreads, SplitShape
           next = page_of(u + run);
         }
         const int id = __shfl_sync(0xffffffffu, cur, (k << pieces_log2) + piece);
-        if (!__all_sync(0xffffffffu, mbar_wait(&empty[stage], phase, abort_flag, a.status))) {
+        if (!__all_sync(0xffffffffu, paged_wait(&empty[stage], phase, flags, a.status))) {
           ok = false;
           break;
         }
@@ -493,7 +551,7 @@ __global__ void __launch_bounds__(SplitShape<D, MT, TEAMS>::kThreads, SplitShape
           if (++stage == Sh::kStages) stage = 0, phase ^= 1u;
           continue;
         }
-        if (!__all_sync(0xffffffffu, mbar_wait(&full[stage], phase, abort_flag, a.status))) {
+        if (!__all_sync(0xffffffffu, paged_wait(&full[stage], phase, flags, a.status))) {
           ok = false;
           break;
         }
@@ -666,9 +724,16 @@ __global__ void __launch_bounds__(SplitShape<D, MT, TEAMS>::kThreads, SplitShape
               const float2 e = *reinterpret_cast<const float2*>(src + k * MT * 8 * Sh::kMergePitch + n * 8);
               v[n][0] += e.x, v[n][1] += e.y;
             }
-          if (r < rows && w.s.n > 1)  // (one token: no row sees what another does not)
-            mend_row<D, F16, kSplitTile, D / 8>(a, v, c2, 8, w.t, w.at, w.at + count, w.i, w.h, w.s.q0 + r / a.G,
-                                                w.h * a.G + r % a.G, lim[x], low[x], top);
+          if (w.s.n > 1)  // (one token: no row sees what another does not)
+            mend_rows(flags, r < rows && odd_columns(v, false), [&] {
+              float f[D / 8][2];
+#pragma unroll
+              for (int n = 0; n < D / 8; ++n) f[n][0] = v[n][0], f[n][1] = v[n][1];
+              mend_row<D, F16, kSplitTile, D / 8>(a, f, c2, 8, w.t, w.at, w.at + count, w.i, w.h, w.s.q0 + r / a.G,
+                                                  w.h * a.G + r % a.G, lim[x], low[x], top);
+#pragma unroll
+              for (int n = 0; n < D / 8; ++n) v[n][0] = f[n][0], v[n][1] = f[n][1];
+            });
           if (r < rows && whole) {
 #pragma unroll
             for (int n = 0; n < D / 8; ++n) *reinterpret_cast<uint32_t*>(dst + n * 8) = pack16<F16>(v[n][0] * inv, v[n][1] * inv);
@@ -955,7 +1020,7 @@ constexpr int kSegRing = 4;
 template <int D, bool F16>
 __global__ void __launch_bounds__(kTileThreads, 1)
     paged_tile_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
-                      const __grid_constant__ CUtensorMap tm_q, const PagedDev a) {
+                      const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ PagedDev a) {
   using Sh = TileShape<D>;
   constexpr int kHalfO = D / 2;  // output columns of a softmax thread
   extern __shared__ uint8_t smem_raw[];
@@ -976,8 +1041,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   uint64_t* seg_empty = bars + 24;  // [kSegRing]
   uint64_t* h_full = bars + 28;   // [tile] the first 32 keys of each half of P
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 30);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  int* slot = reinterpret_cast<int*>(tmem_slot + 2);  // open_range: 4 + 20 words
+  volatile int* flags = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  int* slot = reinterpret_cast<int*>(tmem_slot + 3);  // open_range: 4 + 20 words
   volatile Segment* ring = reinterpret_cast<volatile Segment*>(smem + Sh::kSeg);
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
@@ -1001,7 +1066,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       mbar_init(&seg_full[s], 1);
       mbar_init(&seg_empty[s], 3 + 2 * kTileSoftmaxWarps);  // warps 0, 1 and 2, softmax
     }
-    *abort_flag = 0;
+    flags[0] = flags[1] = 0;
     fence_mbar_init();
   }
   pdl_wait();
@@ -1028,7 +1093,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   auto v_ptr = [&](int st) { return smem + Sh::kV0 + st * Sh::kOperand; };
   // segment number n of the CTA, or a segment that is not valid when a wait gave up
   auto seg_wait = [&](uint32_t n) -> bool {
-    const bool ok = mbar_wait(&seg_full[n & (kSegRing - 1)], (n / kSegRing) & 1, abort_flag, a.status);
+    const bool ok = paged_wait(&seg_full[n & (kSegRing - 1)], (n / kSegRing) & 1, flags, a.status);
     return ok && ring[n & (kSegRing - 1)].valid;
   };
   auto kv_next = [](int kv0, int sink_end, int main0) { return kv0 + kTileN == sink_end ? main0 : kv0 + kTileN; };
@@ -1058,7 +1123,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     auto load_v = [&]() {  // V of the last tile issued, where it is still owed
       if (!v_owed) return;
       const int st = (n_k - 1) & 1;
-      ok = ok && __all_sync(0xffffffffu, mbar_wait(&v_empty[st], (((n_k - 1) >> 1) & 1) ^ 1u, abort_flag, a.status));
+      ok = ok && __all_sync(0xffffffffu, paged_wait(&v_empty[st], (((n_k - 1) >> 1) & 1) ^ 1u, flags, a.status));
       if (ok) load(&tm_v, v_ptr(st), v_id, v_place, v_h, v_edge ? &v_raw[st] : &v_full[st]);
       v_owed = false;
     };
@@ -1086,7 +1151,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         const int id = next, kv1 = kv_next(kv0, sink_end, main0);
         next = t + 1 < n ? page_of(kv1) : -1;
         const int st = n_k & 1, place = (kv0 + lane * box) & (page - 1);
-        ok = __all_sync(0xffffffffu, mbar_wait(&k_empty[st], ((n_k >> 1) & 1) ^ 1u, abort_flag, a.status));
+        ok = __all_sync(0xffffffffu, paged_wait(&k_empty[st], ((n_k >> 1) & 1) ^ 1u, flags, a.status));
         if (!ok) break;
         load(&tm_k, k_ptr(st), id, place, h, &k_full[st]);
         load_v();
@@ -1112,7 +1177,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     uint32_t base = 0, q_n = 0, p_n[2] = {0u, 0u}, o_n[2] = {0u, 0u};  // tiles, q loads, P and O so far
     bool ok = true;
     auto wait = [&](uint64_t* bar, uint32_t parity) {
-      ok = ok && __all_sync(0xffffffffu, mbar_wait(bar, parity & 1u, abort_flag, a.status));
+      ok = ok && __all_sync(0xffffffffu, paged_wait(bar, parity & 1u, flags, a.status));
     };
     auto commit = [&](uint64_t* bar) {
       if (elect_one()) umma_commit(bar);
@@ -1215,7 +1280,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       for (int t = 0; t < n; ++t) {
         const int st = (base + t) & 1;
         if (edge(kv0, lmin, lmax)) {
-          ok = __all_sync(0xffffffffu, mbar_wait(&v_raw[st], seen[st]++ & 1u, abort_flag, a.status));
+          ok = __all_sync(0xffffffffu, paged_wait(&v_raw[st], seen[st]++ & 1u, flags, a.status));
           if (!ok) break;
           for (int key = lane >> 3; key < kTileN; key += 4) {
             const int kv = kv0 + key;
@@ -1241,7 +1306,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       bool ok = true, more = true;
       for (uint32_t seg = 0; ok; ++seg) {
         volatile Segment* sg = ring + (seg & (kSegRing - 1));
-        if (seg >= kSegRing) ok = mbar_wait(&seg_empty[seg & (kSegRing - 1)], (seg / kSegRing - 1) & 1, abort_flag, a.status);
+        if (seg >= kSegRing) ok = paged_wait(&seg_empty[seg & (kSegRing - 1)], (seg / kSegRing - 1) & 1, flags, a.status);
         if (!ok) break;
         const int tok0 = b.rb * 2 * a.tile_tok, toks = min(b.s.n - tok0, 2 * a.tile_tok), n = b.t.main == 0 ? 0 : b.taken;
         sg->valid = more;
@@ -1262,7 +1327,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         mbar_arrive(&seg_full[seg & (kSegRing - 1)]);
         if (!more) break;
         if (n > 0) {
-          if (q_n > 0) ok = mbar_wait(q_empty, (q_n - 1) & 1, abort_flag, a.status);
+          if (q_n > 0) ok = paged_wait(q_empty, (q_n - 1) & 1, flags, a.status);
           if (!ok) break;
           ++q_n;
           const int tiles = toks > a.tile_tok ? 2 : 1;
@@ -1299,7 +1364,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       }
       float m_run = -INFINITY, l_run = 0.0f;
       for (int t = 0; t < work; ++t, ++s_n) {
-        if (!__all_sync(0xffffffffu, mbar_wait(&s_full[g], s_n & 1, abort_flag, a.status))) {
+        if (!__all_sync(0xffffffffu, paged_wait(&s_full[g], s_n & 1, flags, a.status))) {
           ok = false;
           break;
         }
@@ -1375,7 +1440,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       }
       // ---- O / l, or this segment's piece of the unit
       const float l_row = l_run + __shfl_xor_sync(0xffffffffu, l_run, 16);
-      if (work > 0 && ok) ok = __all_sync(0xffffffffu, mbar_wait(&o_full[g], o_n++ & 1, abort_flag, a.status));
+      if (work > 0 && ok) ok = __all_sync(0xffffffffu, paged_wait(&o_full[g], o_n++ & 1, flags, a.status));
       if (!ok) break;
       tc_fence_after();
       const bool stored = r < a.tile_tok * a.G && tok < sg->toks;
@@ -1401,7 +1466,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         bool finite = true;
 #pragma unroll
         for (int i = 0; i < 32; ++i) finite = finite && isfinite(__uint_as_float(o[i]));
-        if (!finite && stored && work > 0) {
+        mend_rows(flags, !finite && stored && work > 0, [&] {
           // (the segment's tiles, counted as tile_at counts them)
           Tiles tl;
           tl.lmin = sg->lmin, tl.lmax = sg->lmax, tl.t0 = sg->main0 / kTileN, tl.main = 1;
@@ -1414,7 +1479,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                                        sg->h * a.G + r % a.G, my_last, my_first, m_run);
 #pragma unroll
           for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(f[i >> 1][i & 1]);
-        }
+        });
         if (stored && whole) {
 #pragma unroll
           for (int i = 0; i < 32; i += 8) {
