@@ -120,6 +120,13 @@ def quantize_weight_tensorwise(w: torch.Tensor) -> tuple[torch.Tensor, torch.Ten
     return q, s
 
 
+def _check_scale(s: torch.Tensor, name: str, like: torch.Tensor) -> None:
+    # the kernels read one fp32 from the device: of a scale for each row they would take row 0's
+    if s.numel() != 1 or s.dtype != torch.float32 or s.device != like.device:
+        raise ValueError(f"qik: {name} is one fp32 scale of the whole tensor on {like.device}, got {tuple(s.shape)} "
+                         f"{s.dtype} on {s.device}")
+
+
 def fp8_gemm(xq: torch.Tensor, sx: torch.Tensor, wq: torch.Tensor, sw: torch.Tensor,
              bias: torch.Tensor | None = None, out_dtype: torch.dtype = torch.bfloat16,
              epilogue: int = L.EPI_SCALE, amax_out: torch.Tensor | None = None,
@@ -134,9 +141,11 @@ def fp8_gemm(xq: torch.Tensor, sx: torch.Tensor, wq: torch.Tensor, sw: torch.Ten
     result is the same).  ``epilogue=EPI_SWIGLU`` takes wq as the fused gate / up
     weight (rows [0, N/2) gate, [N/2, N) up) and returns silu(gate) * up, [M, N/2]
     bf16, the bytes fused_swiglu gives on the two halves of the plain GEMM's output."""
-    lib = L.load()
     if xq.dtype != torch.float8_e4m3fn or wq.dtype != torch.float8_e4m3fn:
         raise TypeError("qik.fp8_gemm: operands must be float8_e4m3fn")
+    _check_scale(sx, "sx", xq)
+    _check_scale(sw, "sw", xq)
+    lib = L.load()
     if xq.stride(-1) != 1:
         xq = xq.contiguous()
     if wq.stride(-1) != 1:
@@ -214,7 +223,8 @@ class FP8Linear(nn.Module):
     def forward_e4m3(self, xq: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
         """forward(x) for an input already quantized as forward(x) would quantize it:
         ``xq`` e4m3 [..., in_features] with its dynamic scale ``scale`` (fp32 [1] on the
-        device), e.g. from ``fused_layer_norm_modulate_e4m3``.  Returns bf16."""
+        device; a scale for each row is refused), e.g. from ``fused_layer_norm_modulate_e4m3``
+        or ``fused_add_rms_norm_e4m3``.  Returns bf16."""
         if xq.dtype != torch.float8_e4m3fn or xq.shape[-1] != self.in_features:
             raise ValueError(f"FP8Linear.forward_e4m3: expected float8_e4m3fn [..., {self.in_features}], "
                              f"got {xq.dtype} {tuple(xq.shape)}")
@@ -253,6 +263,7 @@ class FP8Linear(nn.Module):
         if self.out_features != 3 * heads * D or self.in_features < 256:
             raise ValueError(f"FP8Linear.forward_qkv_rms_rope_e4m3: out_features {self.out_features} is not "
                              f"3 x {heads} heads x {D}")
+        _check_scale(scale, "scale", xq)
         B, S, K = xq.shape
         x2 = xq.reshape(B * S, K)
         if x2.stride(-1) != 1 or x2.stride(0) % 16:
@@ -402,8 +413,7 @@ def fp8_ffn_gelu(x: torch.Tensor, up: FP8Linear, down: FP8Linear, workspace: tor
     status = L.status_word(x.device)
     with torch.cuda.device(x.device):
         if x_scale is not None:
-            if x_scale.dtype != torch.float32 or x_scale.device != x.device:
-                raise ValueError("qik.fp8_ffn_gelu: x_scale must be an fp32 tensor on x's device")
+            _check_scale(x_scale, "x_scale", x)
             L.check(lib.qik_fp8_ffn_e4m3(x2.data_ptr(), x_scale.data_ptr(), M, K, hidden, up.weight.data_ptr(),
                                          up.weight_scale.data_ptr(), L.ptr(b_up), down.weight.data_ptr(),
                                          down.weight_scale.data_ptr(), L.ptr(b_down), y.data_ptr(),

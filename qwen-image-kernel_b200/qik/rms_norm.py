@@ -30,6 +30,6 @@ def fused_add_rms_norm_e4m3(x: torch.Tensor, residual: torch.Tensor | None, weig
                             scales: str = "tensor") -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """As ``fused_add_rms_norm`` with the norm quantized: returns (codes e4m3 [..., N],
     scale fp32, x + residual).  ``scales="tensor"``: one scale, shape [1], which
-    ``FP8Linear.forward_e4m3`` takes; ``scales="row"``: one for each row, shape [...].  NaN in the
-    norm reaches its scale."""
+    ``FP8Linear.forward_e4m3`` takes; ``scales="row"``: one for each row, shape [...] (the linears
+    of this library take one scale only and refuse them).  NaN in the norm reaches its scale."""
     return _calls.add_rms_norm(x, residual, weight, eps, scales or "")

@@ -33,6 +33,7 @@ import torch
 import torch.distributed as dist
 
 from . import _lib as L
+from .fp8 import _check_scale
 
 ROW_ALIGN = 256   # rows per owner are a multiple of the GEMM's tallest tile
 _ALIGN = 256      # byte alignment of the workspace regions
@@ -156,6 +157,7 @@ class PeerRowReduce:
                              f"[{self.M}, *] x [{self.N}, *]")
         if xq.dtype != torch.float8_e4m3fn or weight.dtype != torch.float8_e4m3fn:
             raise TypeError("PeerRowReduce: e4m3 operands only")
+        _check_scale(sx, "sx", xq)
         xq = xq.contiguous()
         self.calls += 1
         parity = self.calls & 1
