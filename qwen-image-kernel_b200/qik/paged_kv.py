@@ -168,15 +168,22 @@ class PagedKVCache:
 
     def truncate(self, seq: int, length: int) -> None:
         """Forget the tokens of ``seq`` behind its first ``length`` (drafted ones that were
-        rejected).  A shared page that is no longer full is copied."""
+        rejected).  A shared page that is no longer full is copied, to a page that the call itself
+        gives up where no other is free; raises CacheFull, with nothing changed, when there is neither."""
         pages = self._pages[self._known(seq)]
         if not 0 <= length <= self._length[seq]:
             raise ValueError(f"qik: PagedKVCache.truncate: {length} tokens of {self._length[seq]}")
         full, rest = divmod(length, self.page_size)
         keep = pages[:full + (1 if rest else 0)]
         if rest and self._users[keep[-1]] > 1:
-            new = self._take(1)[0]
-            self._copy([(keep[-1], new, rest)], [new])
+            own = [p for p in pages[full + 1:] if self._users[p] == 1]
+            if self._free or not own:
+                new = self._take(1)[0]
+                self._copy([(keep[-1], new, rest)], [new])
+            else:
+                new = own[0]
+                self._copy([(keep[-1], new, rest)], [])
+                self._users[new] += 1  # (it stays the sequence's)
             self._drop(pages[full:])
             keep[-1] = new
         else:
