@@ -11,7 +11,6 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
-#include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -20,6 +19,9 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
+#include <cmath>
+#include <numeric>
 #include <string>
 #include <vector>
 
@@ -351,11 +353,49 @@ PyObject* rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
 }
 
 // ---------------------------------------------------------------- attention
-// (Strided views that interleave in one allocation share no element: torch cannot tell, and they pass.)
-bool overlap(const at::Tensor& a, const at::Tensor& b) {
-  const at::MemOverlapStatus s = at::get_overlap_status(a, b);
-  return s == at::MemOverlapStatus::Full || s == at::MemOverlapStatus::Partial ||
-         (s == at::MemOverlapStatus::TooHard && a.data_ptr() == b.data_ptr());
+// Where a tensor's rows are, in bytes: its address, what it spans, a row's columns, the greatest common
+// divisor of the other dims' strides (of those with more than one entry; 0: a single row), the largest
+// of them and what one entry of its dim spans.
+struct Rows {
+  int64_t at, bytes, cols, step, outer, inner;
+};
+Rows rows_in_memory(const at::Tensor& t) {
+  const int64_t e = t.element_size();
+  const bool unit = t.stride(-1) == 1;
+  Rows r = {reinterpret_cast<int64_t>(t.data_ptr()), 0, unit ? t.size(-1) * e : e, 0, 0, 0};
+  if (t.numel() == 0) return r;
+  r.bytes = r.cols;
+  int64_t n = 0;
+  for (int64_t i = 0; i < t.dim() - (unit ? 1 : 0); ++i) {
+    if (t.size(i) < 2) continue;
+    const int64_t s = t.stride(i) * e;
+    r.bytes += (t.size(i) - 1) * s;
+    r.step = std::gcd(r.step, s);
+    if (s > r.outer) r.outer = s, n = t.size(i);
+  }
+  r.inner = r.bytes - (n ? (n - 1) * r.outer : 0);
+  return r;
+}
+// Whether a and b share memory, unless it can be shown that they do not: their spans are apart, or
+// all their rows lie at two places of one period that are apart (columns or heads next to each other
+// in one allocation), or what they hold of each entry of a common outer stride is apart.
+bool overlap(const Rows& a, const Rows& b) {
+  if (a.bytes == 0 || b.bytes == 0 || a.at + a.bytes <= b.at || b.at + b.bytes <= a.at) return false;
+  auto apart = [&](int64_t period, int64_t size_a, int64_t size_b) {
+    if (period == 0) return false;
+    const int64_t d = ((b.at - a.at) % period + period) % period;
+    return d >= size_a && d + size_b <= period;
+  };
+  return !apart(std::gcd(a.step, b.step), a.cols, b.cols) && !(a.outer == b.outer && apart(a.outer, a.inner, b.inner));
+}
+// Whether two entries of t [T, H, D] may share memory.
+bool overlaps_itself(const at::Tensor& t) {
+  const int64_t T = t.size(0), H = t.size(1);
+  int64_t n[2] = {T, H}, s[2] = {T > 1 ? t.stride(0) : 0, H > 1 ? t.stride(1) : 0};
+  if (t.numel() == 0) return false;
+  if (s[0] < s[1]) std::swap(n[0], n[1]), std::swap(s[0], s[1]);
+  const int64_t span = t.size(2) + (n[1] - 1) * s[1];
+  return (n[1] > 1 && s[1] < t.size(2)) || (n[0] > 1 && s[0] < span);
 }
 
 // paged_attention(q, k_pages, v_pages, page_table, seq_lens, query_starts, max_new, max_kv, sm_scale,
@@ -411,7 +451,8 @@ PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
       if (o.stride(2) != 1 || ((o.stride(0) | o.stride(1)) & 7) || !aligned(o))
         refuse(PyExc_ValueError, "qik: out needs a unit column stride, strides of 16 bytes and 16-byte alignment");
       // a row's place is written while other CTAs still read rows
-      if (at::has_internal_overlap(o) == at::MemOverlap::Yes || overlap(o, q0) || overlap(o, kp) || overlap(o, vp))
+      const Rows mem = rows_in_memory(o);
+      if (overlaps_itself(o) || overlap(mem, rows_in_memory(q0)) || overlap(mem, rows_in_memory(kp)) || overlap(mem, rows_in_memory(vp)))
         refuse(PyExc_ValueError, "qik: out overlaps itself, q or the pages");
     }
     const at::Tensor table = table0.stride(1) == 1 || r.W <= 1 ? table0 : table0.contiguous();

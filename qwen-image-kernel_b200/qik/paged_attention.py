@@ -35,7 +35,8 @@ def paged_attention(
     only) those with t > kv - n + j - window or t < ``sinks``.  A row that sees nothing is 0.
     Places that no row of a sequence sees may hold anything, NaN included.  ``sm_scale`` is
     D ** -0.5 by default.  ``out`` ([T, HQ, D], unit column stride) receives the result and may share
-    no memory with q or the pages; rows behind query_starts[B] are not written.  No sequence may bring more than ``max_new``
+    no memory with q or the pages (other heads or tokens of q's allocation are fine; a view that cannot be
+    told apart from what is read is refused); rows behind query_starts[B] are not written.  No sequence may bring more than ``max_new``
     tokens; ``max_kv`` only chooses launch shapes.  Lengths, starts and page numbers outside
     their tensors are skipped and set ``STATUS_BAD_INDEX`` (``qik._lib.device_status``)."""
     return _calls.paged_attention(q, k_pages, v_pages, page_table, seq_lens, query_starts, max_new, max_kv, sm_scale,
