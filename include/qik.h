@@ -36,7 +36,7 @@ extern "C" {
 /* Device-side status word values (written to `status` when non-NULL). */
 #define QIK_STATUS_OK 0
 #define QIK_STATUS_TIMEOUT 1
-#define QIK_STATUS_BAD_INDEX 2 /* a position, slot, page or length outside its tensor (skipped) */
+#define QIK_STATUS_BAD_INDEX 2 /* a position, slot, page or length outside its tensor (skipped); does not replace a timeout */
 
 /* Library version (major*10000 + minor*100 + patch). */
 int qik_version(void);

@@ -34,6 +34,11 @@ __device__ __forceinline__ uint64_t globaltimer() {
   return t;
 }
 
+// Reports an index outside its tensor.  A wait that gave up before stays reported: results may be missing.
+__device__ __forceinline__ void report_bad_index(int* status) {
+  if (status) atomicCAS(status, QIK_DEV_OK, QIK_DEV_BAD_INDEX);
+}
+
 // ---------------------------------------------------------------- mbarrier
 __device__ __forceinline__ void mbar_init(uint64_t* bar, uint32_t count) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(count) : "memory");

@@ -75,8 +75,8 @@ __device__ __forceinline__ Seq seq_of(const PagedDev& a, int i) {
 __device__ __forceinline__ void report_bad_lengths(const PagedDev& a) {
   for (int i = threadIdx.x; i < a.B; i += blockDim.x) {
     const int q0 = __ldg(a.starts + i), q1 = __ldg(a.starts + i + 1), kv = __ldg(a.lens + i);
-    if ((q0 < 0 || q1 < q0 || q1 > a.T || q1 - q0 > a.max_new || kv < 0 || kv > (a.W << a.page_log2)) && a.status)
-      atomicExch(a.status, QIK_DEV_BAD_INDEX);
+    if (q0 < 0 || q1 < q0 || q1 > a.T || q1 - q0 > a.max_new || kv < 0 || kv > (a.W << a.page_log2))
+      report_bad_index(a.status);
   }
 }
 // Last and first key of token j (without the sinks); last < 0: none.
@@ -475,7 +475,7 @@ __global__ void __launch_bounds__(SplitShape<D, MT, TEAMS>::kThreads, SplitShape
         const int p = key >> a.page_log2;
         if (key >= w.s.kv || p >= a.W) return -1;
         const int id = __ldg(row + p);
-        if ((id < 0 || id >= a.pages) && a.status) atomicExch(a.status, QIK_DEV_BAD_INDEX);
+        if (id < 0 || id >= a.pages) report_bad_index(a.status);
         return id < a.pages ? id : -1;
       };
       int cur = 0, next = page_of(w.at);
@@ -1143,7 +1143,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         const int p = key >> a.page_log2;
         if (key >= kv || p >= a.W) return -1;
         const int id = __ldg(row + p);
-        if ((id < 0 || id >= a.pages) && a.status) atomicExch(a.status, QIK_DEV_BAD_INDEX);
+        if (id < 0 || id >= a.pages) report_bad_index(a.status);
         return id < a.pages ? id : -1;
       };
       int next = n > 0 ? page_of(kv0) : -1;

@@ -95,9 +95,9 @@ __global__ void __launch_bounds__(kRotaryWarps * 32) rotary_kernel(const RotaryD
   if (a.paged) {
     slot = load_index(a.slots, t, a.slot64);
     store = slot >= 0 && slot < a.n_slots && pos_ok;
-    if (slot >= a.n_slots && a.status && lane == 0) atomicExch(a.status, QIK_DEV_BAD_INDEX);
+    if (slot >= a.n_slots && lane == 0) report_bad_index(a.status);
   }
-  if (!pos_ok && a.status && lane == 0) atomicExch(a.status, QIK_DEV_BAD_INDEX);
+  if (!pos_ok && lane == 0) report_bad_index(a.status);
   const int64_t pg = store && a.paged ? slot >> a.page_log2 : 0;
   const int64_t in_page = store && a.paged ? slot & ((1 << a.page_log2) - 1) : t;
 

@@ -158,7 +158,8 @@ _status: dict[int, torch.Tensor] = {}
 
 
 def status_word(device: torch.device) -> torch.Tensor:
-    """Per-device int32 status word the kernels write on a failed bounded wait."""
+    """Per-device int32 status word the kernels write: STATUS_TIMEOUT on a bounded wait that gave up,
+    STATUS_BAD_INDEX on an index outside its tensor (which never replaces a timeout)."""
     idx = device.index if device.index is not None else torch.cuda.current_device()
     t = _status.get(idx)
     if t is None:
@@ -179,7 +180,8 @@ def status_ptr(idx: int) -> int:
 
 
 def device_status(device: torch.device | None = None) -> int:
-    """Read (synchronizing) the device status word; 0 means no kernel gave up a wait."""
+    """Read (synchronizing) the device status word; 0 means that no kernel gave up a wait or met an
+    index outside its tensor since the word was last cleared."""
     dev = device or torch.device("cuda", torch.cuda.current_device())
     return int(status_word(dev)[0].item())
 
