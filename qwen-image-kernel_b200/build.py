@@ -8,7 +8,8 @@ dependency beyond the driver.  Objects are rebuilt when their source or any head
 is newer.
 
 The host calls of the decoder operators (csrc/calls.cpp) are a CPython module over torch's
-C++ tensors, compiled by g++ to qik/_calls.so and linked against libqik.so beside it.
+C++ tensors, compiled by g++ to qik/_calls.so and linked against libqik.so beside it; it is made again
+when the Python or the torch that it was compiled against is another one.
 """
 from __future__ import annotations
 
@@ -25,6 +26,7 @@ OBJ = CSRC / "_build"
 INCLUDE = HERE.parent / "include"
 OUT = HERE / "qik" / "libqik.so"
 CALLS = HERE / "qik" / "_calls.so"
+CALLS_MADE_FOR = OBJ / "_calls.made_for"   # the Python and torch that _calls.so was compiled against
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr", "-Xptxas",
@@ -69,7 +71,9 @@ def build_calls(force: bool = False) -> Path:
 
     import torch
     src, header = CSRC / "calls.cpp", INCLUDE / "qik.h"
-    if not force and CALLS.exists() and CALLS.stat().st_mtime >= max(src.stat().st_mtime, header.stat().st_mtime):
+    made_for = f"Python {sys.version} ({sysconfig.get_config_var('SOABI')}), torch {torch.__version__} ({torch.version.git_version})"
+    if (not force and CALLS.exists() and CALLS.stat().st_mtime >= max(src.stat().st_mtime, header.stat().st_mtime)
+            and CALLS_MADE_FOR.exists() and CALLS_MADE_FOR.read_text() == made_for):
         return CALLS
     root = Path(torch.__file__).resolve().parent
     cuda = Path(nvcc()).resolve().parent.parent
@@ -79,7 +83,10 @@ def build_calls(force: bool = False) -> Path:
            "-L", str(root / "lib"), "-ltorch_python", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda",
            "-L", str(OUT.parent), "-l:libqik.so", "-Wl,-rpath,$ORIGIN"]
     print("[qik build] g++", src.name, flush=True)
+    CALLS_MADE_FOR.unlink(missing_ok=True)
     subprocess.run(cmd, check=True)
+    OBJ.mkdir(parents=True, exist_ok=True)
+    CALLS_MADE_FOR.write_text(made_for)
     return CALLS
 
 
