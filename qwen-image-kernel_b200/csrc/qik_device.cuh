@@ -85,6 +85,13 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volati
   }
 }
 
+// After a wait gave up: a millisecond for the CTA's copies and matrix instructions in flight to land
+// before its shared and tensor memory go to another CTA.
+__device__ __forceinline__ void let_land() {
+  const uint64_t t0 = globaltimer();
+  while (globaltimer() - t0 < 1000000ull) __nanosleep(1000);
+}
+
 // ---------------------------------------------------------------- TMA
 __device__ __forceinline__ void tma_prefetch_desc(const CUtensorMap* m) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(m)) : "memory");

@@ -750,6 +750,7 @@ __global__ void __launch_bounds__(SplitShape<D, MT, TEAMS>::kThreads, SplitShape
       more = walk_next(a, w, count);
     }
   }
+  if (flags[0]) let_land();
   pdl_trigger();
 }
 
@@ -1503,6 +1504,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       if (lane == 0) mbar_arrive(&seg_empty[seg & (kSegRing - 1)]);
     }
   }
+  if (flags[0]) let_land();
   tc_fence_before();
   __syncthreads();
   pdl_trigger();
