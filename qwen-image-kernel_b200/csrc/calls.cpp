@@ -255,8 +255,14 @@ PyObject* copy_pages(PyObject*, PyObject* const* a, Py_ssize_t n) {
     p.k = k.data_ptr(), p.v = v.data_ptr();
     p.layers = at ? k.size(0) : 1;
     p.pages = k.size(at), p.heads = k.size(at + 1), p.page = k.size(at + 2), p.token_bytes = k.size(at + 3) * size;
-    if (k.stride(at + 3) != 1 || v.stride(at + 3) != 1 || k.stride(at + 2) != k.size(at + 3) || v.stride(at + 2) != k.size(at + 3))
-      refuse(PyExc_ValueError, "qik: a head's tokens must be contiguous in a page");
+    const int64_t D = k.size(at + 3), H = p.heads;
+    auto tokens_together = [&](const at::Tensor& t) { return t.stride(at + 3) == 1 && t.stride(at + 2) == D; };
+    // [pages, page, heads, D] seen with its heads first: the first tokens of a page are one run of all heads
+    auto heads_together = [&](const at::Tensor& t) { return t.stride(at + 3) == 1 && t.stride(at + 1) == D && t.stride(at + 2) == H * D; };
+    const bool whole = !tokens_together(k) && heads_together(k) && heads_together(v);
+    if (!whole && !(tokens_together(k) && tokens_together(v)))
+      refuse(PyExc_ValueError, "qik: copy_pages: in a page the tokens of a head, or the heads of a token, must be contiguous, the same in both pools");
+    if (whole) p.heads = 1, p.token_bytes *= H;
     p.k_layer_bytes = at ? k.stride(0) * size : 0, p.v_layer_bytes = at ? v.stride(0) * size : 0;
     p.k_page_bytes = k.stride(at) * size, p.v_page_bytes = v.stride(at) * size;
     p.k_head_bytes = k.stride(at + 1) * size, p.v_head_bytes = v.stride(at + 1) * size;

@@ -27,8 +27,9 @@ def copy_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, moves) -> None:
     """Copy the first tokens of pages to other pages, in every layer and head of both pools.
 
     k_pages, v_pages: [layers, pages, heads, page, D] (or one layer's [pages, heads, page, D]);
-    moves: a list of (from, to, tokens), or an int array or tensor [n, 3].  The rest of a
-    written page stays as it is.  No page may be written twice or both read and written in one
+    moves: a list of (from, to, tokens), or an int array or tensor [n, 3].  In a page the tokens of a
+    head are contiguous, or the heads of a token and then the tokens (a pool [pages, page, heads, D] seen
+    with its heads first); other strides are refused.  The rest of a written page stays as it is.  No page may be written twice or both read and written in one
     call; indices are checked before anything is launched."""
     if not isinstance(moves, (list, tuple)):
         moves = moves.tolist()
