@@ -562,12 +562,16 @@ int qik_copy_pages(const qik_page_pools* pools, const int32_t* moves, int64_t n,
  *   A new token at place p of its sequence sees the keys t <= p (QIK_PAGED_CAUSAL) or all
  *   seq_lens[i] of them; with window > 0 (causal only) those with t > p - window or
  *   t < sinks.  out = softmax(q . k * sm_scale) . v; a row that sees no key is 0.  Whatever
- *   the unseen places of a page hold has no effect where no row of the call's sequence
- *   sees them.
+ *   the places that a row does not see hold has no effect on it (rows before infinities or NaN
+ *   that others of their tile see are formed a second time, key by key).  Scores, sums and
+ *   the accumulated output are fp32; the probabilities are rounded to the tensors' type for the
+ *   product with v, and the result once.
  *   q, out [T, HQ, D] with element strides (token, head); k_pages, v_pages [pages, HK, page,
  *   D] with element strides (page, head, token); unit column strides; bf16, or fp16 with
  *   QIK_PAGED_F16; query head h reads key head h / (HQ / HK).  page_table [B, W] int32
  *   with row stride table_st.  Rows of out behind query_starts[B] are not written.
+ *   query_starts ascend from 0 to T at most: a sequence whose start lies below the one before
+ *   is reported, and rows of that call may stay unwritten.
  *   max_new, max_kv: upper bounds (host) of n_i and seq_lens[i]; they choose launch shapes,
  *   and no sequence may exceed max_new.
  *   ws: qik_paged_attention_workspace_bytes(args) bytes, 16-byte aligned, not initialised by

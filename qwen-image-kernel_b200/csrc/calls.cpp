@@ -116,8 +116,8 @@ int* status_of(int device) {
 void* stream_of(int device) { return c10::cuda::getCurrentCUDAStream(static_cast<c10::DeviceIndex>(device)).stream(); }
 
 // ---------------------------------------------------------------- RMS norm
-// t ([..., N]) with one row pitch, copied only where its leading dims do not flatten to rows
-// of one pitch or the alignment is not 16 bytes.
+// t ([..., N]) with one row pitch: contiguous tensors and rows [M, N] of a pitch as they are, copied where
+// the alignment is not 16 bytes and where there are more dims that are not contiguous.
 at::Tensor rows_of(const at::Tensor& t, int64_t N, int64_t& pitch) {
   pitch = N;
   if (t.is_contiguous()) return aligned(t) ? t : t.clone(at::MemoryFormat::Contiguous);

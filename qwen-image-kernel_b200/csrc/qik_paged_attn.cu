@@ -5,9 +5,10 @@
 // over the keys j of the row's sequence that it sees: j <= limit (its own place in the
 // sequence; the last key when not causal), and with a window j > limit - window or
 // j < sinks.  m_i is the running maximum of an online softmax; scores, maxima, sums and
-// the output accumulate in fp32, p is rounded to the tensors' type before p . v (its
-// relative error, 2^-9 in bf16 and 2^-12 in fp16 at most, averages over the keys, and the
-// sum uses the unrounded p).  A row that sees no key is 0.
+// the output accumulate in fp32.  p is rounded to the tensors' type before p . v, the operand
+// of the 16-bit matrix instructions: a relative error of 2^-8 in bf16 and 2^-11 in fp16 at
+// most (there up to 2^-25 absolute below 2^-14), which averages over the keys; the sum uses
+// the unrounded p.  A row that sees no key is 0.
 //
 // The `group` query heads that share a key head are packed as rows: row r of a (sequence,
 // key head) is token r / group, head r % group, so each K/V tile is read once for the
@@ -22,7 +23,7 @@
 //   to a workspace and are joined by paged_join_kernel in a fixed order.  Two
 //   TMA warps fill a ring of K and V tiles; 8 warps split the tiles, their keys and the
 //   16-row groups between them and run mma.sync m16n8k16: tcgen05's 128-row tiles would be
-//   8 to 87% padding here and the tensor pipe is not what bounds it.
+//   50 to 99% padding here and the tensor pipe is not what bounds it.
 //
 //   paged_tile_kernel (more rows: chunks and prompts).  Bound by the tensor core: two
 //   128-row query tiles on tcgen05 share every 128-key tile, as in qik_attn.cu.
@@ -1016,7 +1017,7 @@ constexpr int kSegRing = 4;
 //               (columns, group heads, tokens), which is the packed row order);
 //   warps 4-19  softmax, eight warps per query tile, two threads a row.
 // Query tile 0 ends earlier than tile 1 under a causal mask: its count of tiles is its own.
-// A prompt of 8001 tokens with 24 heads of 128: 402 us, 977 TFLOP/s of the pairs that are seen; the tensor pipe
+// A prompt of 8001 tokens with 24 heads of 128: 402 to 419 us by the clock, up to 977 TFLOP/s of the pairs that are seen; the tensor pipe
 // and the special function unit are each 59% busy, the rest is the wait of a tile for its own product.
 template <int D, bool F16>
 __global__ void __launch_bounds__(kTileThreads, 1)

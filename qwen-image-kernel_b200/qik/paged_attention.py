@@ -33,11 +33,17 @@ def paged_attention(
     The new tokens are the last of their sequence, already stored.  Row j of n in a sequence of
     ``kv`` tokens sees the keys t <= kv - n + j (``causal``) or all kv; with ``window`` (causal
     only) those with t > kv - n + j - window or t < ``sinks``.  A row that sees nothing is 0.
-    Places that no row of a sequence sees may hold anything, NaN included.  ``sm_scale`` is
-    D ** -0.5 by default.  ``out`` ([T, HQ, D], unit column stride) receives the result and may share
-    no memory with q or the pages (other heads or tokens of q's allocation are fine; a view that cannot be
-    told apart from what is read is refused); rows behind query_starts[B] are not written.  No sequence may bring more than ``max_new``
-    tokens; ``max_kv`` only chooses launch shapes.  Lengths, starts and page numbers outside
-    their tensors are skipped and set ``STATUS_BAD_INDEX`` (``qik._lib.device_status``)."""
+    Places that a row does not see may hold anything, NaN included (a row that others of its
+    tile see infinities beside is formed a second time, which takes longer).  ``sm_scale`` is
+    D ** -0.5 by default.  Sums are fp32; the probabilities are rounded to q's type before the
+    product with v, as the matrix instructions take them.
+
+    ``out`` ([T, HQ, D], unit column stride) receives the result and may share no memory with q
+    or the pages: other heads or tokens of q's allocation are fine, a view that cannot be told
+    apart from what is read is refused.  Rows behind query_starts[B] are not written.
+
+    ``query_starts`` ascend; no sequence may bring more than ``max_new`` tokens; ``max_kv`` only
+    chooses launch shapes.  Lengths, starts and page numbers outside their tensors are skipped
+    and set ``STATUS_BAD_INDEX`` (``qik._lib.device_status``)."""
     return _calls.paged_attention(q, k_pages, v_pages, page_table, seq_lens, query_starts, max_new, max_kv, sm_scale,
                                   causal, window, sinks, out)
